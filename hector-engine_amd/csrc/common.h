@@ -286,6 +286,18 @@ int he_attention_prefill_wide(void* out, const void* q, const void* kpool, const
                               int max_q_len, int total_rows, int H, int KVH, int hd, int window, float scale,
                               int parts, float* ws_o, float* ws_ml, const AttnExtras& ex, void* stream);
 
+// gemm_tall.hip: a routed feed-forward's rows in groups, one an expert: whole tiles of bm slots each, its rows in their order
+#define HE_GROUP_ROWS_MOST 1024     // groups
+struct GroupRows {
+  const int32_t* tile_begin;   // [groups + 1] a group's first tile
+  const int32_t* rows_of;      // a slot's row, -1: none
+  const float* scale;          // the weight of a slot's choice
+  const int32_t* choice_of;    // a slot's place in the row-by-row list of choices, -1: none
+  const int32_t* slot_of;      // a choice's slot, -1: its id is no group's
+};
+int64_t he_group_rows_ints(int rows, int top, int groups, int bm);
+int he_group_rows(GroupRows* lists, void* scratch_i32, const void* ids_i32, const void* weights_f32, int rows, int top, int groups, int bm, void* stream);
+
 #define HE_REQUIRE(cond, ...)      \
   do {                             \
     if (!(cond)) {                 \

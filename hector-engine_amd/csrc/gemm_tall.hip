@@ -65,7 +65,7 @@ extern "C" int he_gemm_tall_tile(int M, int N, int K, int slices) {
 // choice went (-1: nowhere).
 // grid: an expert a workgroup, each counts all of them (a few thousand ids from L2) and writes its own.
 #define GR_THREADS 1024
-#define GR_MAX_GROUPS 1024
+#define GR_MAX_GROUPS HE_GROUP_ROWS_MOST
 __global__ __launch_bounds__(GR_THREADS) void group_rows_kernel(int32_t* __restrict__ tile_begin, int32_t* __restrict__ rows_of,
                                                                 float* __restrict__ scale, int32_t* __restrict__ slot_of,
                                                                 int32_t* __restrict__ choice_of, const int32_t* __restrict__ ids,
@@ -120,6 +120,22 @@ static int gr_most_tiles(int64_t choices, int groups, int bm) {
 extern "C" int he_group_rows_most_tiles(int rows, int top, int groups, int bm) {
   return rows <= 0 || top <= 0 || groups <= 0 || bm <= 0 ? 0 : gr_most_tiles((int64_t)rows * top, groups, bm);
 }
+// the lists in scratch of he_group_rows_ints ints
+int64_t he_group_rows_ints(int rows, int top, int groups, int bm) {
+  return (groups + 1 + 3) / 4 * 4 + 3ll * bm * he_group_rows_most_tiles(rows, top, groups, bm) + (int64_t)rows * top;
+}
+int he_group_rows(GroupRows* lists, void* scratch_i32, const void* ids_i32, const void* weights_f32, int rows, int top, int groups, int bm, void* stream) {
+  const int slots = bm * gr_most_tiles((int64_t)rows * top, groups, bm);
+  int32_t* tile_begin = (int32_t*)scratch_i32;
+  int32_t* rows_of = tile_begin + (groups + 1 + 3) / 4 * 4;
+  float* scale = (float*)(rows_of + slots);
+  int32_t* choice_of = (int32_t*)(scale + slots);
+  int32_t* slot_of = choice_of + slots;
+  *lists = {tile_begin, rows_of, scale, choice_of, slot_of};
+  group_rows_kernel<<<groups, GR_THREADS, 0, (hipStream_t)stream>>>(tile_begin, rows_of, scale, slot_of, choice_of, (const int32_t*)ids_i32,
+                                                                    (const float*)weights_f32, rows * top, top, groups, bm);
+  return he_check_launch("he_group_rows");
+}
 
 // out[row][d] = the sum over the row's choices that an expert took (slot_of) of partial[row][choice][d], in their order, + dense[row][groups] * x[row][d]
 // (x null: without).
@@ -156,7 +172,7 @@ __global__ __launch_bounds__(256) void combine_groups_kernel(uint16_t* __restric
 // down null: the activations alone, h_bf16 [rows][real I] with expert e's columns from e I on, the chosen ones written (the
 // caller has cleared it); out, partial and dense are not used.
 extern "C" int64_t he_routed_groups_ints(int rows, int top, int real, int bm) {
-  return (real + 1 + 3) / 4 * 4 + 3ll * bm * he_group_rows_most_tiles(rows, top, real, bm) + (int64_t)rows * top;
+  return he_group_rows_ints(rows, top, real, bm);
 }
 extern "C" int he_routed_groups(void* out, void* lists_i32, void* h_bf16, void* partial_f32, const void* x, const void* gate_up,
                                 const void* down, int64_t ldw, const void* ids_i32, const void* weights_f32,
@@ -174,25 +190,19 @@ extern "C" int he_routed_groups(void* out, void* lists_i32, void* h_bf16, void* 
   if (rows == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
   const int mtiles = gr_most_tiles((int64_t)rows * top, real, bm), slots = bm * mtiles;
-  int32_t* tile_begin = (int32_t*)lists_i32;
-  int32_t* rows_of = tile_begin + (real + 1 + 3) / 4 * 4;
-  float* scale = (float*)(rows_of + slots);
-  int32_t* choice_of = (int32_t*)(scale + slots);
-  int32_t* slot_of = choice_of + slots;
-  group_rows_kernel<<<real, GR_THREADS, 0, s>>>(tile_begin, rows_of, scale, slot_of, choice_of, (const int32_t*)ids_i32,
-                                                (const float*)weights_f32, rows * top, top, real, bm);
-  int rc = he_check_launch("he_routed_groups (lists)");
+  GroupRows lists;
+  int rc = he_group_rows(&lists, lists_i32, ids_i32, weights_f32, rows, top, real, bm, stream);
   if (rc) return rc;
   const GatedAct act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic};
   const GtCase up = {(const uint16_t*)x, (const uint16_t*)gate_up, h_bf16, nullptr, 0, slots, 2 * I, D, D, D, spread ? (int64_t)real * I : I, (int64_t)2 * I * D,
-               tile_begin, rows_of, scale, nullptr, real, spread, act, 1, -1, false};
-  const GtCase dn = {(const uint16_t*)h_bf16, (const uint16_t*)down, partial_f32, nullptr, 0, slots, D, I, I, ldw, D, I, tile_begin,
-               nullptr, nullptr, choice_of, real, 0, act, 1, -1, false};
+               lists.tile_begin, lists.rows_of, lists.scale, nullptr, real, spread, act, 1, -1, false};
+  const GtCase dn = {(const uint16_t*)h_bf16, (const uint16_t*)down, partial_f32, nullptr, 0, slots, D, I, I, ldw, D, I, lists.tile_begin,
+               nullptr, nullptr, lists.choice_of, real, 0, act, 1, -1, false};
   rc = gt_launch(up, bm << 16 | 256, mtiles, GT_GATED, s);
   if (rc || spread) return rc;
   rc = gt_launch(dn, bm << 16 | 256, mtiles, GT_F32, s);
   if (rc) return rc;
-  combine_groups_kernel<<<dim3((D + 1023) / 1024, rows), 256, 0, s>>>((uint16_t*)out, (const float*)partial_f32, slot_of,
+  combine_groups_kernel<<<dim3((D + 1023) / 1024, rows), 256, 0, s>>>((uint16_t*)out, (const float*)partial_f32, lists.slot_of,
                                                                       (const float*)dense_f32, identity ? (const uint16_t*)x : nullptr,
                                                                       top, real, D);
   return he_check_launch("he_routed_groups (sum)");

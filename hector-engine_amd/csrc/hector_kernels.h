@@ -6,7 +6,7 @@
 #pragma once
 #include <stdint.h>
 
-#define HE_ABI_VERSION 31
+#define HE_ABI_VERSION 32
 
 #ifdef __cplusplus
 extern "C" {
@@ -448,6 +448,27 @@ int he_latent_cache(void* q_out, int64_t q_out_row, void* kpool, void* vpool, co
                     const void* row_seq, const void* seq_slot, const void* page_table, int max_blocks, int num_pages,
                     const void* inv_freq, int interleaved, float mscale, int rows, int H, int d, int r, int rank, int pd,
                     int dtype, void* stream);
+
+// ---- weights in 4 bits (fp4.h) -------------------------------------------------
+// codes [matrices][ceil(N / 16)][ceil(K / 128)][1024 bytes] and scales bf16 [matrices][ceil(N / 16)][ceil(K / 128)][128 / group][16] of
+// w [matrices][N][K], rows ldw apart (float32 or bfloat16); group 32, 64 or 128.
+int he_fp4_pack(void* codes, void* scales, const void* w, int64_t ldw, int matrices, int N, int K, int group, int dtype, void* stream);
+// out [matrices][N][K] = the values of a packed matrix (exact in bfloat16)
+int he_fp4_unpack(void* out, const void* codes, const void* scales, int matrices, int N, int K, int group, int dtype, void* stream);
+// out[M][N] (float32 or bfloat16, rows ldo apart) = x[M][K] (bfloat16, rows ldx apart) . W^T (+ bias); gated: bf16 [M][N / 2] of a weight
+// that alternates gate and up rows, the activation's constants as he_gated_act takes them. workspace: he_fp4_product_workspace_bytes.
+int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int gated);
+int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M, int N,
+                   int K, int group, int out_dtype, int bias_dtype, int gated, float alpha, float limit, float up_shift, float cubic,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+// A routed feed-forward over packed experts: out[row] (bf16 [rows][D]) = the sum over the row's choices (ids [rows][top], the expert; an id
+// that is none adds nothing) of weights[row][choice] * down_e act(gate_e x, up_e x). up: matrices of [2 I, D], gate and up rows in
+// turn; down: matrices of [D, I].
+int64_t he_fp4_experts_workspace_bytes(int rows, int top, int experts, int I, int D);
+int he_fp4_experts(void* out, const void* x, int64_t ldx, const void* up_codes, const void* up_scales, const void* down_codes,
+                   const void* down_scales, const void* ids_i32, const void* weights_f32, int rows, int top, int experts, int I, int D,
+                   int group_up, int group_down, float alpha, float limit, float up_shift, float cubic, void* workspace,
+                   int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

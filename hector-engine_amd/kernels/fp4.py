@@ -1,0 +1,69 @@
+"""Weights in 4 bits: the packed matrix, and packing one.
+
+A matrix [N, K] (or several of one size, [E, N, K]) is kept as codes of 4 bits, a sign and one of the magnitudes
+0, 0.5, 1, 1.5, 2, 3, 4, 6, and one scale for every `group` (32, 64 or 128) neighbours along K:
+
+    scale = max |w| / 6, rounded to six significant bits          code = the nearest to w / scale, ties to the even one
+
+so that scale * code is a bfloat16 number exactly, and a group's largest magnitude is off by at most a sixty-fourth
+of it. A group of zeros has scale 0; one that holds a NaN or an infinity has a NaN scale, and every value of it is NaN.
+4.125, 4.25 or 4.5 bits a value where bfloat16 has 16. (The reference's compact formats keep 4 to 5 bits a value: tools/quant_bench/README.md:305-307.)
+
+The tiles' layout is the kernels' own (csrc/fp4.h): a packed matrix is read by ops.fp4_product, ops.fp4_experts and unpack().
+"""
+from __future__ import annotations
+
+import torch
+
+GROUPS = (32, 64, 128)
+TILE_ROWS, TILE_K = 16, 128
+
+
+class Fp4Weight:
+    """A packed matrix; `shape` is the matrix's. Made by pack()."""
+
+    dtype = "fp4"      # what a table of kernel routes looks it up by
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple, group: int):
+        self.codes, self.scales, self.shape, self.group = codes, scales, tuple(shape), group
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.scales.nbytes
+
+    def dim(self) -> int:
+        return len(self.shape)
+
+    def unpack(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values, bfloat16 (exact) or float32."""
+        from . import ops
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        ops.fp4_unpack(out, self)
+        return out
+
+
+def storage_shapes(shape: tuple, group: int) -> tuple[tuple, tuple]:
+    """The shapes of the codes (uint8) and the scales (bfloat16) of a matrix [N, K], or of several [E, N, K]."""
+    if len(shape) not in (2, 3) or any(s <= 0 for s in shape):
+        raise ValueError(f"fp4: a matrix is [N, K] or [E, N, K] of positive sizes, not {tuple(shape)}")
+    if group not in GROUPS:
+        raise ValueError(f"fp4: groups of {group}, must be one of {GROUPS}")
+    *lead, n, k = shape
+    tiles = (*lead, -(-n // TILE_ROWS), -(-k // TILE_K))
+    return (*tiles, TILE_ROWS * TILE_K // 2), (*tiles, TILE_K // group, TILE_ROWS)
+
+
+def pack(w: torch.Tensor, group: int = 64) -> Fp4Weight:
+    """Packs a float32 or bfloat16 matrix on the GPU (the rows of a matrix [N, K] may lie apart)."""
+    from . import ops
+    codes, scales = storage_shapes(tuple(w.shape), group)
+    if not w.is_cuda:
+        raise ValueError("fp4.pack: expected a GPU tensor")
+    packed = Fp4Weight(torch.empty(codes, dtype=torch.uint8, device=w.device),
+                       torch.empty(scales, dtype=torch.bfloat16, device=w.device), tuple(w.shape), group)
+    ops.fp4_pack(packed, w)
+    return packed

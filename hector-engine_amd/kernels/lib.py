@@ -16,7 +16,7 @@ _lib = None
 
 _CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
 
-EXPECTED_ABI = 31
+EXPECTED_ABI = 32
 
 c_int, c_i64, c_f32, c_ptr = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -116,6 +116,14 @@ _SIGNATURES = {
                          c_int, c_int, c_int, c_f32, c_f32, c_f32, c_f32, c_ptr],
     "he_chosen_experts": [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int,
                           c_int, c_int, c_f32, c_f32, c_f32, c_f32, c_int, c_ptr],
+    "he_fp4_pack": [c_ptr, c_ptr, c_ptr, c_i64, c_int, c_int, c_int, c_int, c_int, c_ptr],
+    "he_fp4_unpack": [c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_ptr],
+    "he_fp4_product_workspace_bytes": [c_int, c_int, c_int, c_int],
+    "he_fp4_product": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32,
+                       c_f32, c_f32, c_ptr, c_i64, c_ptr],
+    "he_fp4_experts_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
+    "he_fp4_experts": [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                       c_f32, c_f32, c_f32, c_f32, c_ptr, c_i64, c_ptr],
     "he_diff_heads": [c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32, c_f32, c_int, c_ptr],
     "he_attention_plain_workspace_floats": [c_int, c_int, c_int, c_int, c_int, c_int],
     "he_attention_plain": [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int,
@@ -157,6 +165,8 @@ _RESTYPES = {
     "he_delta_workspace_floats": c_i64,
     "he_gemm_plain_workspace_floats": c_i64,
     "he_routed_groups_ints": c_i64,
+    "he_fp4_product_workspace_bytes": c_i64,
+    "he_fp4_experts_workspace_bytes": c_i64,
     "he_attention_decode_workspace_floats": c_i64,
     "he_attention_decode_fused_workspace_floats": c_i64,
     "he_attention_prefill_workspace_floats": c_i64,

@@ -1393,6 +1393,154 @@ def chosen_experts(out, h_scratch, x, gate_up, down, ids, weights, dense, rows: 
                                    _stream()))
 
 
+def _fp4_here(name: str, *tensors) -> None:
+    """Tensors (None allowed) of one GPU, the current one: a launch goes to its stream."""
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name}: expected GPU tensors")
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name}: a tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _fp4_weight(name: str, w, dims: int = 2) -> None:
+    from .fp4 import Fp4Weight, storage_shapes
+    if not isinstance(w, Fp4Weight):
+        raise TypeError(f"{name}: expected a packed weight (kernels.fp4.pack), got {type(w).__name__}")
+    codes, scales = storage_shapes(w.shape, w.group)
+    _need(w.codes, f"{name}: codes", torch.uint8, codes)
+    _need(w.scales, f"{name}: scales", torch.bfloat16, scales)
+    if w.dim() != dims:
+        raise ValueError(f"{name}: expected a packed weight of {dims} dims, got {w.shape}")
+    _fp4_here(name, w.codes, w.scales)
+
+
+def _fp4_rows(name: str, t, what: str, rows: int, cols: int, dtype) -> None:
+    """[rows or more, cols] whose elements of a row are neighbours; the rows may lie apart."""
+    _fp4_here(name, t)
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: {what} is {t.dtype}, expected {dtype}")
+    if t.dim() != 2 or t.shape[1] != cols or t.shape[0] < rows:
+        raise ValueError(f"{name}: {what}{tuple(t.shape)} is not [{rows}, {cols}]")
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name}: {what}'s rows must be contiguous and must not overlap, strides {t.stride()}")
+
+
+def _fp4_row_stride(t, cols: int) -> int:
+    return t.stride(0) if t.shape[0] > 1 else cols
+
+
+def _fp4_workspace(name: str, workspace, size: int):
+    if size == 0:
+        return None, 0
+    if workspace is None:
+        raise ValueError(f"{name}: a workspace of {size} bytes is needed")
+    _need(workspace, f"{name}: workspace", torch.uint8)
+    _fp4_here(name, workspace)
+    if workspace.numel() < size or workspace.data_ptr() % 16:
+        raise ValueError(f"{name}: a workspace of {size} bytes, 16-byte aligned, is needed; got {workspace.numel()}")
+    return workspace.data_ptr(), workspace.numel()
+
+
+@_op("fp4_pack")
+def fp4_pack(packed, w) -> None:
+    """packed (kernels.fp4.Fp4Weight) = w, float32 or bfloat16, of its shape."""
+    _fp4_weight("fp4_pack", packed, packed.dim())
+    _fp4_here("fp4_pack", w)
+    if tuple(w.shape) != packed.shape:
+        raise ValueError(f"fp4_pack: w{tuple(w.shape)} for a packed weight of {packed.shape}")
+    *lead, N, K = packed.shape
+    ld = w.stride(-2) if N > 1 else K
+    if (K > 1 and w.stride(-1) != 1) or ld < K or (lead and lead[0] > 1 and w.stride(0) != N * ld):
+        raise ValueError(f"fp4_pack: w's rows must be contiguous and lie evenly, strides {w.stride()}")
+    _lib.check(_lib.load().he_fp4_pack(packed.codes.data_ptr(), packed.scales.data_ptr(), w.data_ptr(), ld, lead[0] if lead else 1, N, K,
+                                       packed.group, dtype_code(w.dtype), _stream()))
+
+
+@_op("fp4_unpack")
+def fp4_unpack(out, packed) -> None:
+    """out (float32 or bfloat16, contiguous) = the values of a packed weight."""
+    _fp4_weight("fp4_unpack", packed, packed.dim())
+    _need(out, "fp4_unpack: out", shape=packed.shape)
+    _fp4_here("fp4_unpack", out)
+    *lead, N, K = packed.shape
+    _lib.check(_lib.load().he_fp4_unpack(out.data_ptr(), packed.codes.data_ptr(), packed.scales.data_ptr(), lead[0] if lead else 1, N, K,
+                                         packed.group, dtype_code(out.dtype), _stream()))
+
+
+def fp4_product_workspace_bytes(rows: int, w, gated: bool = False) -> int:
+    """Bytes of scratch memory that fp4_product wants for this weight and so many rows (0: none)."""
+    return int(_lib.load().he_fp4_product_workspace_bytes(rows, *w.shape, int(gated)))
+
+
+@_op("fp4_product")
+def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.0, 0.0), workspace=None) -> None:
+    """out[rows, N] (bfloat16 or float32) = x[rows, K] (bfloat16) . W^T (+ bias [N]) with a packed weight (kernels.fp4), sums in 32 bits;
+    or, gated, out[rows, N / 2] (bfloat16, no bias) = act(gate, up) for a weight that alternates gate and up rows, act =
+    (alpha, limit, up_shift[, cubic]) the activation's constants as silu_mul takes them. The rows of x and out may lie apart.
+    workspace: uint8, fp4_product_workspace_bytes(rows, w, gated) or more; calls that may run at the same time need one each."""
+    _fp4_weight("fp4_product", w)
+    N, K = w.shape
+    if rows < 0:
+        raise ValueError(f"fp4_product: {rows} rows")
+    if gated and (N % 2 or bias is not None):
+        raise ValueError("fp4_product: a gated product has an even number of weight rows and no bias")
+    _fp4_rows("fp4_product", x, "x", rows, K, torch.bfloat16)
+    if out.dtype not in ((torch.bfloat16,) if gated else (torch.bfloat16, torch.float32)):
+        raise TypeError(f"fp4_product: results in {out.dtype}")
+    cols = N // 2 if gated else N
+    _fp4_rows("fp4_product", out, "out", rows, cols, out.dtype)
+    if bias is not None:
+        _need(bias, "fp4_product: bias", shape=(N,))
+        _fp4_here("fp4_product", bias)
+    ws, size = _fp4_workspace("fp4_product", workspace, fp4_product_workspace_bytes(rows, w, gated))
+    if rows == 0:
+        return
+    _lib.check(_lib.load().he_fp4_product(
+        out.data_ptr(), _fp4_row_stride(out, cols), x.data_ptr(), _fp4_row_stride(x, K), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), rows,
+        N, K, w.group, dtype_code(out.dtype), dtype_code(bias.dtype) if bias is not None else F32, int(gated), *_act4(act), ws, size,
+        _stream()))
+
+
+def fp4_experts_workspace_bytes(rows: int, top: int, gate_up, down) -> int:
+    """Bytes of scratch memory that fp4_experts wants for so many rows of `top` choices."""
+    E, D, I = down.shape
+    return int(_lib.load().he_fp4_experts_workspace_bytes(rows, top, E, I, D))
+
+
+@_op("fp4_experts")
+def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0, 0.0), workspace=None) -> None:
+    """A routed feed-forward over packed experts: out[rows, D] (bfloat16) = the sum over a row's choices c of weights[row, c] *
+    down[e] act(gate[e] x, up[e] x) with e = ids[row, c]; an id that is no expert adds nothing, nor does a weight of 0. gate_up: packed
+    [E, 2 I, D], gate i of an expert in row 2 i, its up in 2 i + 1; down: packed [E, D, I]; ids int32, weights float32
+    [rows, top]; x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. workspace: uint8,
+    fp4_experts_workspace_bytes(rows, top, gate_up, down) or more; calls that may run at the same time need one each."""
+    _fp4_weight("fp4_experts", gate_up, 3)
+    _fp4_weight("fp4_experts", down, 3)
+    E, D, I = down.shape
+    if gate_up.shape != (E, 2 * I, D):
+        raise ValueError(f"fp4_experts: gate_up{gate_up.shape} for down{down.shape}, expected {(E, 2 * I, D)}")
+    if rows < 0:
+        raise ValueError(f"fp4_experts: {rows} rows")
+    _fp4_rows("fp4_experts", x, "x", rows, D, torch.bfloat16)
+    _need(out, "fp4_experts: out", torch.bfloat16)
+    _fp4_rows("fp4_experts", out, "out", rows, D, torch.bfloat16)
+    _need(ids, "fp4_experts: ids", torch.int32)
+    _need(weights, "fp4_experts: weights", torch.float32)
+    _fp4_here("fp4_experts", ids, weights)
+    if ids.dim() != 2 or ids.shape[0] < rows or ids.shape[1] == 0 or weights.shape != ids.shape:
+        raise ValueError(f"fp4_experts: ids{tuple(ids.shape)} and weights{tuple(weights.shape)} are not [{rows}, choices]")
+    top = ids.shape[1]
+    ws, size = _fp4_workspace("fp4_experts", workspace, fp4_experts_workspace_bytes(rows, top, gate_up, down))
+    if rows == 0:
+        return
+    _lib.check(_lib.load().he_fp4_experts(
+        out.data_ptr(), x.data_ptr(), _fp4_row_stride(x, D), gate_up.codes.data_ptr(), gate_up.scales.data_ptr(), down.codes.data_ptr(),
+        down.scales.data_ptr(), ids.data_ptr(), weights.data_ptr(), rows, top, E, I, D, gate_up.group, down.group, *_act4(act), ws, size,
+        _stream()))
+
+
 @_op("diff_heads")
 def diff_heads(out, attn, rows: int, H: int, G: int, hd: int, vd: int, lam: float, post: float, eps: float) -> None:
     """out[rows, H, vd] = rms(a1 - lam * a2) * post per head, a1 and a2 the outputs of the two score maps in

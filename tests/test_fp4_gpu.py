@@ -1,0 +1,353 @@
+"""Weights in 4 bits on the GPU: packing, the product and a routed feed-forward over packed experts, against their definitions in
+float64 (tests/plain/fp4_plain.py). A bfloat16 result is off by half a step (2^-8 of the value at most) and the sum's own bound."""
+import pytest
+import torch
+
+from tests.plain import fp4_plain as P
+
+pytestmark = pytest.mark.gpu
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+HALF = {BF16: 2.0 ** -8, F32: 2.0 ** -24}
+
+
+@pytest.fixture(scope="module")
+def api():
+    import hector_engine_amd  # noqa: F401
+    from hector_engine_amd.kernels import fp4, ops
+    return fp4, ops
+
+
+def rnd(seed, *shape, scale=1.0, dtype=BF16):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=gen) * scale).to(dtype)
+
+
+def workspace(size):
+    return torch.full((size,), 0xFF, dtype=torch.uint8, device="cuda")      # (stale memory is NaN)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("shape", [(1, 1), (16, 128), (17, 129), (5, 31), (3, 33, 200), (2, 16, 96), (40, 264), (1000, 1003)])
+def test_packing_gives_the_nearest_values(api, shape, group, dtype):
+    fp4, _ = api
+    w = rnd(1, *shape, scale=0.02, dtype=dtype)
+    packed = fp4.pack(w.cuda(), group)
+    want = P.values(w, group)
+    assert torch.equal(packed.unpack(F32).cpu().double(), want)
+    assert torch.equal(packed.unpack().cpu().double(), want)      # exact in bfloat16 too
+
+
+def test_packing_borders_zeros_and_numbers_that_are_none(api):
+    fp4, _ = api
+    w = torch.zeros(8, 64)
+    # scale 1 (largest magnitude 6): every border between two magnitudes, both signs, and their neighbours
+    border = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    w[0, :7], w[0, 7:14], w[0, 14] = border, -border, 6.0
+    w[1, :7], w[1, 7:14], w[1, 14] = torch.nextafter(border, torch.tensor(9.0)), torch.nextafter(border, torch.tensor(0.0)), -6.0
+    w[2, 5] = float("nan")
+    w[3, 40] = float("inf")
+    w[4, 0], w[4, 1] = 3.4e38, -3.4e38             # six times the scale is still a number
+    w[5, :3] = torch.tensor([1e-38, -1e-39, 1e-45])
+    w[6, :] = -0.0
+    w[7, 0] = 6 * (1 + 1 / 64)                     # a scale between two of six bits: the even one
+    packed = fp4.pack(w.cuda(), 32)
+    got = packed.unpack(F32).cpu()
+    assert got[0, :15].tolist() == [0, 1, 1, 2, 2, 4, 4, 0, -1, -1, -2, -2, -4, -4, 6]
+    assert got[1, :15].tolist() == [0.5, 1, 1.5, 2, 3, 4, 6, 0, 0.5, 1, 1.5, 2, 3, 4, -6]
+    assert got[2, :32].isnan().all() and not got[2, 32:].isnan().any()
+    assert got[3, 32:].isnan().all() and not got[3, :32].isnan().any()
+    assert got[4].isfinite().all() and 3.3e38 < got[4, 0] <= 3.4e38 and got[4, 1] == -got[4, 0]
+    assert got[5, 0] == pytest.approx(1e-38, rel=1 / 32) and got[5, 3:].abs().max() == 0
+    assert got[6].abs().max() == 0 and got[7, 0] == 6.0
+
+
+def test_packing_rows_that_lie_apart(api):
+    fp4, _ = api
+    wide = rnd(2, 50, 300, scale=0.02).cuda()
+    for cut in (wide[:, :128], wide[:, 3:200], wide[::2, 8:136]):
+        assert torch.equal(fp4.pack(cut, 64).unpack(), fp4.pack(cut.contiguous(), 64).unpack())
+
+
+SIZES = [(1, 16, 128), (1, 1, 8), (2, 17, 40), (1, 300, 1003), (4, 64, 256), (5, 130, 2056), (16, 48, 1152), (16, 4608, 384),
+         (17, 1001, 1003), (32, 96, 136), (33, 200, 520), (64, 256, 1024), (65, 80, 264), (130, 36, 640), (200, 530, 384), (300, 2050, 1160)]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_product(api, M, N, K, group):
+    fp4, ops = api
+    x, w, b = rnd(3, M, K), rnd(4, N, K, scale=0.05), rnd(5, N)
+    packed = fp4.pack(w.cuda(), group)
+    values = P.values(w, group)
+    want = x.double() @ values.T
+    bound = P.sum_bound(x, values, group)
+    for dtype, bias in ((F32, None), (BF16, None), (F32, b), (BF16, b.float())):
+        out = torch.full((M + 1, N), float("nan"), dtype=dtype, device="cuda")
+        ops.fp4_product(out, x.cuda(), packed, None if bias is None else bias.cuda(), M,
+                        workspace=workspace(ops.fp4_product_workspace_bytes(M, packed)))
+        exact = want if bias is None else want + bias.double()
+        got = out.cpu().double()
+        assert got[M].isnan().all()                  # the row behind the last is left as it was
+        # (the bias's addition and the last rounding: half a step each)
+        assert ((got[:M] - exact).abs() <= bound * (1 + HALF[dtype]) + (HALF[dtype] + 2.0 ** -24) * (exact.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("act", [(1.0, 0.0, 0.0), (1.702, 7.0, 1.0)])
+@pytest.mark.parametrize("M,N,K", [(1, 2, 32), (3, 34, 200), (16, 512, 384), (17, 130, 136), (64, 320, 1024), (130, 258, 264), (260, 1028, 520)])
+def test_gated_product(api, M, N, K, act):
+    fp4, ops = api
+    x, w = rnd(6, M, K), rnd(7, N, K, scale=0.1)
+    packed = fp4.pack(w.cuda(), 64)
+    values = P.values(w, 64)
+    z, bound = x.double() @ values.T, P.sum_bound(x, values, 64)
+    out = torch.full((M + 1, N // 2), float("nan"), dtype=BF16, device="cuda")
+    ops.fp4_product(out, x.cuda(), packed, None, M, gated=True, act=act, workspace=workspace(ops.fp4_product_workspace_bytes(M, packed, True)))
+    exact = P.act(z, *act)
+    # |d act / d gate| <= 1.13 (|up| + shift), |d act / d up| <= |gate| (x * sigmoid(a x) for a >= 1 grows by at most 1.1 a step); its own
+    # evaluation in 32 bits is off by a few last places, and by 2^-24 alpha |gate| where the exponential's argument is rounded
+    g, u = z[:, 0::2].abs(), z[:, 1::2].abs()
+    slack = 1.13 * bound[:, 0::2] * (u + bound[:, 1::2] + act[2]) + (g + bound[:, 0::2]) * bound[:, 1::2] + 2.0 ** -20 * g * (u + act[2]) * (1 + g)
+    got = out.cpu().double()
+    assert got[M].isnan().all()
+    assert ((got[:M] - exact).abs() <= slack + HALF[BF16] * (exact.abs() + slack) + 2.0 ** -120).all()
+
+
+def test_product_of_rows_that_lie_apart(api):
+    """Rows at a distance, a base that is not 16-byte aligned, an output inside a wider tensor: the same bits."""
+    fp4, ops = api
+    w = fp4.pack(rnd(8, 100, 264, scale=0.05).cuda(), 32)
+    for M in (1, 7, 40, 150):
+        wide = rnd(9, M, 700).cuda()
+        for c0 in (0, 8, 3):
+            cut = wide[:, c0:c0 + 264]
+            size = ops.fp4_product_workspace_bytes(M, w)
+            want = torch.empty((M, 100), dtype=F32, device="cuda")
+            ops.fp4_product(want, cut.contiguous(), w, None, M, workspace=workspace(size))
+            room = torch.full((M, 170), 7.0, device="cuda")
+            ops.fp4_product(room[:, 5:105], cut, w, None, M, workspace=workspace(size))
+            assert torch.equal(room[:, 5:105], want)
+            assert (room[:, :5] == 7).all() and (room[:, 105:] == 7).all()
+
+
+def test_a_row_without_numbers_stays_alone(api):
+    """NaN and infinities in a row of x, and NaN groups of a weight row, reach their own row and column and no others."""
+    fp4, ops = api
+    for M in (3, 16, 40, 130):
+        w = rnd(10, 40, 200, scale=0.05)
+        x = rnd(11, M, 200)
+        clean = torch.empty((M, 40), dtype=F32, device="cuda")
+        size = workspace(ops.fp4_product_workspace_bytes(M, fp4.pack(w.cuda(), 64)))
+        ops.fp4_product(clean, x.cuda(), fp4.pack(w.cuda(), 64), None, M, workspace=size)
+        x[1, 5], x[2, 199] = float("nan"), float("inf")
+        w[7, 100] = float("nan")
+        got = torch.empty_like(clean)
+        ops.fp4_product(got, x.cuda(), fp4.pack(w.cuda(), 64), None, M, workspace=size)
+        keep = torch.ones((M, 40), dtype=torch.bool)
+        keep[1:3], keep[:, 7] = False, False
+        assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
+        assert got[1].isnan().all() and got[:, 7].isnan().all() and not got[2].isfinite().any()
+
+
+def experts_case(seed, rows, E, top, I, D, group, act, holes=True):
+    gu, dn, x = rnd(seed, E, 2 * I, D, scale=0.1), rnd(seed + 1, E, D, I, scale=0.1), rnd(seed + 2, rows, D)
+    gen = torch.Generator().manual_seed(seed + 3)
+    ids = torch.randint(0, max(1, E - 1), (rows, top), generator=gen, dtype=torch.int32)     # (the last expert has no row)
+    shares = torch.rand((rows, top), generator=gen)
+    if holes and rows > 1:
+        ids[rows // 2, 0] = -1
+        ids[rows - 1, :] = E + 3                     # a row none of whose choices is an expert
+        shares[0, top - 1] = 0.0
+    wu, wd = P.values(gu, group), P.values(dn, group)
+    exact, slack = torch.zeros((rows, D), dtype=F64), torch.zeros((rows, D), dtype=F64)
+    for r in range(rows):
+        for c in range(top):
+            e = int(ids[r, c])
+            if not 0 <= e < E:
+                continue
+            s = float(shares[r, c])
+            z, bound = x[r:r + 1].double() @ wu[e].T, P.sum_bound(x[r:r + 1], wu[e], group)
+            h = s * P.act(z, *act)
+            # as the gated product's slack; the activations times their share are rounded to bfloat16 for the second product
+            g, u = z[:, 0::2].abs(), z[:, 1::2].abs()
+            d = s * (1.13 * bound[:, 0::2] * (u + bound[:, 1::2] + act[2]) + (g + bound[:, 0::2]) * bound[:, 1::2]
+                     + 2.0 ** -20 * g * (u + act[2]) * (1 + g))
+            d = d + HALF[BF16] * (h.abs() + d)
+            exact[r] += (h @ wd[e].T)[0]
+            slack[r] += (d @ wd[e].abs().T + P.sum_bound(h.abs() + d, wd[e], group))[0] * (1 + top * 2.0 ** -24)
+    return gu, dn, x, ids, shares, exact, slack
+
+
+@pytest.mark.parametrize("rows,E,top,I,D,group,act", [
+    (1, 2, 1, 8, 16, 32, (1.0, 0.0, 0.0)), (1, 16, 4, 40, 64, 64, (1.0, 0.0, 0.0)), (5, 8, 3, 24, 72, 32, (1.702, 7.0, 1.0)),
+    (20, 3, 3, 136, 128, 128, (1.0, 0.0, 0.0)), (64, 4, 2, 64, 200, 32, (1.0, 0.0, 0.0)), (130, 2, 2, 48, 40, 64, (1.0, 0.0, 0.0)),
+    (150, 7, 2, 20, 36, 32, (1.702, 7.0, 1.0)), (3, 200, 8, 8, 16, 32, (1.0, 0.0, 0.0)), (400, 3, 2, 144, 264, 128, (1.0, 0.0, 0.0))])
+def test_experts(api, rows, E, top, I, D, group, act):
+    fp4, ops = api
+    gu, dn, x, ids, shares, exact, slack = experts_case(20, rows, E, top, I, D, group, act)
+    up, down = fp4.pack(gu.cuda(), group), fp4.pack(dn.cuda(), group)
+    out = torch.full((rows + 1, D), float("nan"), dtype=BF16, device="cuda")
+    ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, act=act,
+                    workspace=workspace(ops.fp4_experts_workspace_bytes(rows, top, up, down)))
+    got = out.cpu().double()
+    assert got[rows].isnan().all()
+    assert ((got[:rows] - exact).abs() <= slack + HALF[BF16] * (exact.abs() + slack)).all()
+    if rows > 1:
+        assert (got[rows - 1] == 0).all()
+
+
+def test_experts_the_same_expert_twice_and_a_row_without_numbers(api):
+    """A row that names one expert twice takes it twice; a NaN row reaches no other row."""
+    fp4, ops = api
+    E, I, D = 4, 24, 64
+    up, down = fp4.pack(rnd(30, E, 2 * I, D, scale=0.1).cuda(), 32), fp4.pack(rnd(31, E, D, I, scale=0.1).cuda(), 32)
+    x = rnd(32, 6, D).cuda()
+
+    def run(x, ids, shares):
+        out = torch.empty((x.shape[0], D), dtype=BF16, device="cuda")
+        ops.fp4_experts(out, x, up, down, ids.cuda(), shares.cuda(), x.shape[0],
+                        workspace=workspace(ops.fp4_experts_workspace_bytes(x.shape[0], ids.shape[1], up, down)))
+        return out
+    once = run(x, torch.full((6, 1), 2, dtype=torch.int32), torch.full((6, 1), 0.5))
+    twice = run(x, torch.full((6, 2), 2, dtype=torch.int32), torch.full((6, 2), 0.25))
+    assert torch.equal(once, twice)                  # 0.25 h + 0.25 h is 0.5 h exactly, in every step of the sums
+    ids = torch.tensor([[0, 1], [1, 2], [2, 3], [3, 0], [0, 2], [1, 3]], dtype=torch.int32)
+    shares = torch.full((6, 2), 0.5)
+    clean = run(x, ids, shares)
+    bad = x.clone()
+    bad[3] = float("nan")
+    got = run(bad, ids, shares)
+    keep = torch.tensor([0, 1, 2, 4, 5])
+    assert torch.equal(got[keep], clean[keep]) and got[3].isnan().all()
+
+
+def test_a_row_does_not_depend_on_the_rows_beside_it(api):
+    """Within one kernel's range of row counts a row has the same bits whatever stands beside it, and run after run."""
+    fp4, ops = api
+    w = fp4.pack(rnd(40, 272, 392, scale=0.05).cuda(), 64)
+    for lo, hi in ((2, 16), (17, 32), (33, 64), (257, 300)):
+        x = rnd(41, hi, 392).cuda()
+        size = workspace(max(ops.fp4_product_workspace_bytes(lo, w), ops.fp4_product_workspace_bytes(hi, w)))
+        a, b = torch.empty((hi, 272), dtype=F32, device="cuda"), torch.empty((hi, 272), dtype=F32, device="cuda")
+        ops.fp4_product(a, x, w, None, hi, workspace=size)
+        ops.fp4_product(b, x, w, None, hi, workspace=size)
+        assert torch.equal(a, b)
+        ops.fp4_product(b, x, w, None, lo, workspace=size)
+        assert torch.equal(a[:lo], b[:lo])
+
+
+def test_replayed_graphs_and_two_streams(api):
+    """Captured calls replay, with eager work between them, on the inputs as they are then; two graphs with a workspace each, and calls on two
+    streams at once, give what one alone gives."""
+    fp4, ops = api
+    E, I, D, rows, top = 4, 64, 128, 9, 2
+    up, down = fp4.pack(rnd(50, E, 2 * I, D, scale=0.1).cuda(), 32), fp4.pack(rnd(51, E, D, I, scale=0.1).cuda(), 32)
+    w = fp4.pack(rnd(52, 96, D, scale=0.1).cuda(), 32)
+    ids = torch.randint(0, E, (rows, top), dtype=torch.int32, device="cuda")
+    shares = torch.rand((rows, top), device="cuda")
+
+    def make():
+        st = dict(x=torch.zeros((rows, D), dtype=BF16, device="cuda"), moe=torch.empty((rows, D), dtype=BF16, device="cuda"),
+                  y=torch.empty((rows, 96), dtype=F32, device="cuda"), ws=workspace(ops.fp4_experts_workspace_bytes(rows, top, up, down)),
+                  ws2=workspace(ops.fp4_product_workspace_bytes(rows, w)))
+
+        def call():
+            ops.fp4_experts(st["moe"], st["x"], up, down, ids, shares, rows, workspace=st["ws"])
+            ops.fp4_product(st["y"], st["moe"], w, None, rows, workspace=st["ws2"])
+        return st, call
+
+    graphs = []
+    for _ in range(2):
+        st, call = make()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        graphs.append((st, g))
+    for turn in range(4):
+        for i, (st, g) in enumerate(graphs):
+            st["x"].copy_(rnd(60 + 2 * turn + i, rows, D))
+            g.replay()
+        ref, call = make()
+        for i, (st, _) in enumerate(graphs):
+            ref["x"].copy_(rnd(60 + 2 * turn + i, rows, D))
+            call()
+            torch.cuda.synchronize()
+            assert torch.equal(ref["y"], st["y"]) and torch.equal(ref["moe"], st["moe"])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    runs = [make(), make()]
+    for i, (st, _) in enumerate(runs):
+        st["x"].copy_(rnd(80 + i, rows, D))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (st, call), s in zip(runs, streams):
+            with torch.cuda.stream(s):
+                call()
+    torch.cuda.synchronize()
+    ref, call = make()
+    for i, (st, _) in enumerate(runs):
+        ref["x"].copy_(rnd(80 + i, rows, D))
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(ref["y"], st["y"])
+
+
+def test_refusals(api):
+    """Wrong sizes, dtypes and layouts are refused on the host, before any launch; nothing is written."""
+    fp4, ops = api
+    w = fp4.pack(rnd(70, 32, 64).cuda(), 32)
+    stack, downs = fp4.pack(rnd(71, 2, 32, 64).cuda(), 32), fp4.pack(rnd(72, 2, 64, 16).cuda(), 32)
+    x, out = rnd(73, 4, 64).cuda(), torch.full((4, 32), 7.0, device="cuda")
+    with pytest.raises(ValueError, match="groups of 48"):
+        fp4.pack(x, 48)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        fp4.pack(x.cpu(), 32)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        fp4.pack(x.half(), 32)
+    with pytest.raises(ValueError, match="positive sizes"):
+        fp4.pack(x[:0], 32)
+    with pytest.raises(ValueError, match="contiguous"):
+        fp4.pack(x.t(), 32)
+    with pytest.raises(TypeError, match="packed weight"):
+        ops.fp4_product(out, x, x, None, 4)
+    with pytest.raises(ValueError, match="2 dims"):
+        ops.fp4_product(out, x, stack, None, 4)
+    with pytest.raises(TypeError, match="x is torch.float32"):
+        ops.fp4_product(out, x.float(), w, None, 4)
+    with pytest.raises(ValueError, match=r"x\(4, 56\)"):
+        ops.fp4_product(out, x[:, :56], w, None, 4)
+    with pytest.raises(ValueError, match=r"is not \[5, 64\]"):
+        ops.fp4_product(out, x, w, None, 5)
+    with pytest.raises(ValueError, match="-1 rows"):
+        ops.fp4_product(out, x, w, None, -1)
+    with pytest.raises(ValueError, match="contiguous and must not overlap"):
+        ops.fp4_product(out, x[:1].expand(4, 64), w, None, 4)
+    with pytest.raises(TypeError, match="results in torch.float16"):
+        ops.fp4_product(out.half(), x, w, None, 4)
+    with pytest.raises(ValueError, match="bias"):
+        ops.fp4_product(out, x, w, torch.zeros(31, device="cuda"), 4)
+    with pytest.raises(ValueError, match="gated"):
+        ops.fp4_product(out[:, :16].to(BF16), x, w, torch.zeros(32, device="cuda"), 4, gated=True)
+    with pytest.raises(TypeError, match="results in torch.float32"):
+        ops.fp4_product(out[:, :16], x, w, None, 4, gated=True)
+    ids, shares = torch.zeros((4, 2), dtype=torch.int32, device="cuda"), torch.zeros((4, 2), device="cuda")
+    moe = torch.full((4, 64), 7.0, dtype=BF16, device="cuda")
+    ws = workspace(ops.fp4_experts_workspace_bytes(4, 2, stack, downs))
+    with pytest.raises(ValueError, match="a workspace of"):
+        ops.fp4_experts(moe, x, stack, downs, ids, shares, 4)
+    with pytest.raises(ValueError, match="a workspace of"):
+        ops.fp4_experts(moe, x, stack, downs, ids, shares, 4, workspace=ws[:-1])
+    with pytest.raises(ValueError, match="expected .2, 32, 64."):
+        ops.fp4_experts(moe, x, downs, downs, ids, shares, 4, workspace=ws)
+    with pytest.raises(TypeError, match="ids: expected torch.int32"):
+        ops.fp4_experts(moe, x, stack, downs, ids.long(), shares, 4, workspace=ws)
+    with pytest.raises(ValueError, match="choices"):
+        ops.fp4_experts(moe, x, stack, downs, ids, shares[:, :1].contiguous(), 4, workspace=ws)
+    ops.fp4_product(out, x, w, None, 0)              # no rows: nothing happens
+    ops.fp4_experts(moe, x, stack, downs, ids, shares, 0, workspace=ws)
+    torch.cuda.synchronize()
+    assert (out == 7).all() and (moe == 7).all()
