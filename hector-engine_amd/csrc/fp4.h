@@ -26,6 +26,15 @@ __device__ __forceinline__ fp4_bf16x8 fp4_operand(uint32_t codes) {
   return fp4_bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// eight codes times their scale, as an operand (exact)
+__device__ __forceinline__ fp4_bf16x8 fp4_values(uint32_t codes, float scale) {
+  const fp4_f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 1);
+  const fp4_f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 3);
+  const uint4 v = make_uint4(pack2_bf16(a[0] * scale, a[1] * scale), pack2_bf16(b[0] * scale, b[1] * scale),
+                             pack2_bf16(c[0] * scale, c[1] * scale), pack2_bf16(d[0] * scale, d[1] * scale));
+  return __builtin_bit_cast(fp4_bf16x8, v);
+}
+
 // A packed matrix, or one per group of rows (the experts of a routed feed-forward).
 struct Fp4Weight {
   const uint8_t* codes;
@@ -42,7 +51,7 @@ struct Fp4Case {
   bool whole;                 // x may be read 16 bytes at a time
   void* out;
   int64_t ldo;
-  bool out_f32, gated, clamped;
+  bool out_f32, gated;
   const void* bias;           // [N] or null
   int bias_dtype;
   int M;
@@ -52,4 +61,76 @@ struct Fp4Case {
   const int32_t* rows_of;     // a slot's row of x, -1: none
   const int32_t* out_of;      // a slot's row of out, -1: none
   const float* factor;        // what a slot's results are multiplied by, or null
+  bool pairs;                 // out takes stores of four neighbouring results (gated: of two)
 };
+
+// The gated activation for results of 8 bits: the hardware's power of two and reciprocal, off by a few last places of 32-bit numbers
+// (2^-22 of the value, and 2^-24 |alpha gate| where the power's argument is rounded), in a third of the instructions of the library's
+// exponential and a division.
+__device__ __forceinline__ float fp4_act(float g, float u, const GatedAct& a) {
+  g = fminf(g, a.limit);
+  u = fminf(fmaxf(u, -a.limit), a.limit);
+  const float z = fmaf(a.cubic, g * g, a.alpha) * g;
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z)) * (u + a.shift);
+}
+
+// a lane's four neighbouring results, columns n to n + 3 of row `to`, times f
+__device__ __forceinline__ void fp4_store(const Fp4Case& c, fp4_f32x4 v, int64_t to, int n, float f) {
+  if (c.gated) {
+    uint16_t* p = (uint16_t*)c.out + to * c.ldo + n / 2;
+    auto act = [&](float g, float u) {
+      return f == 0.f ? 0.f : fp4_act(g, u, c.act) * f;    // (a choice without weight adds nothing, whatever its row holds)
+    };
+    const uint32_t pair = pack2_bf16(act(v[0], v[1]), act(v[2], v[3]));
+    if (c.pairs && n + 4 <= c.w.N) {
+      *reinterpret_cast<uint32_t*>(p) = pair;
+    } else {
+      p[0] = (uint16_t)pair;
+      if (n + 2 < c.w.N) p[1] = (uint16_t)(pair >> 16);
+    }
+    return;
+  }
+  if (c.bias)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += load_param(c.bias, min(n + e, c.w.N - 1), c.bias_dtype);
+  if (c.out_f32) {
+    float* p = (float*)c.out + to * c.ldo + n;
+    if (c.pairs && n + 4 <= c.w.N) {
+      *reinterpret_cast<fp4_f32x4*>(p) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < c.w.N) p[e] = v[e];
+    }
+    return;
+  }
+  uint16_t* p = (uint16_t*)c.out + to * c.ldo + n;
+  const uint32_t a = pack2_bf16(v[0], v[1]), b = pack2_bf16(v[2], v[3]);
+  if (c.pairs && n + 4 <= c.w.N) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < c.w.N) p[e] = (uint16_t)((e < 2 ? a : b) >> (16 * (e & 1)));
+  }
+}
+
+// the group of rows that tile `tile` belongs to: the last one that begins at or before it
+__device__ __forceinline__ int fp4_group_of(const int32_t* tile_begin, int groups, int tile) {
+  int lo = 0, hi = groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tile_begin[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// fp4_few.hip: rows in tiles of 16
+int fp4_run_few(const Fp4Case& c, int mtiles, hipStream_t s);
+// fp4_tall.hip: rows in tiles of 16 mt, mtiles of them at most, weight rows in tiles of 64 nt; x may be read 16 bytes at a time, K is a multiple of
+// 128. slices > 1: K cut in so many (of a block at least), their sums by way of parts [slices][M][N rounded up to 16].
+struct Fp4Plan {
+  int mt, nt, slices;
+};
+int fp4_run_tall(const Fp4Case& c, Fp4Plan plan, int mtiles, float* parts, hipStream_t s);
