@@ -78,6 +78,9 @@ def parse_args(argv: list[str]):
                     help="a prompt as token ids; repeat for a batch")
     ap.add_argument("--tokens-file", default=None, help="a file with one prompt of token ids a line")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default="stored", choices=["stored", "fp4"],
+                    help="fp4: the layers' matrices are packed into 4 bits when they are loaded (bfloat16 only)")
+    ap.add_argument("--weight-group", type=int, default=64, choices=[32, 64, 128], help="with --weights fp4: neighbours that share a scale")
     ap.add_argument("--stop-ids", default=None, help="comma-separated stop token ids")
     ap.add_argument("--no-graph", action="store_true", help="run one-token steps without HIP graphs")
     ap.add_argument("--tune-gemm", action="store_true",
@@ -177,7 +180,7 @@ def main(argv: list[str] | None = None) -> int:
     pages = slots * ((ctx + 63) // 64)
     start = time.perf_counter()
     source = dict(config=config, seed=ns.seed) if ns.random is not None else dict(model_dir=model)
-    engine = he.Engine(dtype=ns.dtype, max_tokens=pages * 64, max_slots=slots, max_seq_len=ctx,
+    engine = he.Engine(dtype=ns.dtype, weights=ns.weights, weight_group=ns.weight_group, max_tokens=pages * 64, max_slots=slots, max_seq_len=ctx,
                        use_graphs=not ns.no_graph, tune_library=ns.tune_gemm, profile=ns.profile,
                        sync_each_launch=ns.sync_each_launch, **source)
     what = f"random weights for {ns.random}, seed {ns.seed}" if ns.random is not None else model

@@ -115,18 +115,32 @@ ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   return t;
 }
 
-// out[row] = the sum over the row's choices, in their order, of those that an expert took
+// out[row] = the sum over the row's choices, in their order, of those that an expert took, and of weight * x of those from `experts` on (x null:
+// they add nothing)
 __global__ __launch_bounds__(256) void add_choices_kernel(uint16_t* __restrict__ out, const float* __restrict__ partial, const int32_t* __restrict__ ids,
-                                                          int top, int experts, int D) {
+                                                          const float* __restrict__ weights, const uint16_t* __restrict__ x, int64_t ldx, int top,
+                                                          int experts, int D) {
   const int64_t row = blockIdx.y;
-  const int d = blockIdx.x * 256 + threadIdx.x;
+  const int d = 4 * (blockIdx.x * 256 + threadIdx.x);
   if (d >= D) return;
-  float sum = 0.f;
+  const int n = min(4, D - d);
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int k = 0; k < top; ++k) {
-    const int id = ids[row * top + k];
-    if (id >= 0 && id < experts) sum += partial[(row * top + k) * D + d];
+    const int64_t choice = row * top + k;
+    const int id = ids[choice];
+    if (id < 0 || (id >= experts && !x)) continue;
+    const float w = weights[choice];
+    if (id >= experts) {
+      if (w == 0.f) continue;
+      for (int i = 0; i < n; ++i) sum[i] = fmaf(w, bf16_bits_to_float(x[row * ldx + d + i]), sum[i]);
+    } else if (D % 4 == 0) {
+      const float4 v = *reinterpret_cast<const float4*>(partial + choice * D + d);
+      sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+    } else {
+      for (int i = 0; i < n; ++i) sum[i] += partial[choice * D + d + i];
+    }
   }
-  out[row * D + d] = float_to_bf16_bits(sum);
+  for (int i = 0; i < n; ++i) out[row * D + d + i] = float_to_bf16_bits(sum[i]);
 }
 
 }  // namespace
@@ -173,7 +187,7 @@ extern "C" int64_t he_fp4_experts_workspace_bytes(int rows, int top, int experts
 
 extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void* up_codes, const void* up_scales, const void* down_codes,
                               const void* down_scales, const void* ids_i32, const void* weights_f32, int rows, int top, int experts, int I, int D,
-                              int group_up, int group_down, float alpha, float limit, float up_shift, float cubic, void* workspace, int64_t workspace_bytes, void* stream) {
+                              int group_up, int group_down, int identity, float alpha, float limit, float up_shift, float cubic, void* workspace, int64_t workspace_bytes, void* stream) {
   HE_REQUIRE(rows >= 0 && top > 0 && experts > 0 && I > 0 && D > 0 && I <= (1 << 25), "he_fp4_experts: bad sizes");
   HE_REQUIRE(experts <= HE_GROUP_ROWS_MOST && rows <= 65535 && (int64_t)rows * top < (1 << 26), "he_fp4_experts: %d experts and %d rows are too many", experts, rows);
   HE_REQUIRE(ldx >= D, "he_fp4_experts: rows of %d at a distance of %lld", D, (long long)ldx);
@@ -215,6 +229,7 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
     }
     if ((rc = fp4_run_tall(up, t.up, t.mtiles, nullptr, s)) || (rc = fp4_run_tall(down, t.down, t.mtiles, nullptr, s))) return rc;
   }
-  add_choices_kernel<<<dim3((D + 255) / 256, rows), 256, 0, s>>>((uint16_t*)out, partial, (const int32_t*)ids_i32, top, experts, D);
+  add_choices_kernel<<<dim3((D + 1023) / 1024, rows), 256, 0, s>>>((uint16_t*)out, partial, (const int32_t*)ids_i32, (const float*)weights_f32,
+                                                                   identity ? (const uint16_t*)x : nullptr, ldx, top, experts, D);
   return he_check_launch("he_fp4_experts");
 }

@@ -462,12 +462,12 @@ int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx, const voi
                    int K, int group, int out_dtype, int bias_dtype, int gated, float alpha, float limit, float up_shift, float cubic,
                    void* workspace, int64_t workspace_bytes, void* stream);
 // A routed feed-forward over packed experts: out[row] (bf16 [rows][D]) = the sum over the row's choices (ids [rows][top], the expert; an id
-// that is none adds nothing) of weights[row][choice] * down_e act(gate_e x, up_e x). up: matrices of [2 I, D], gate and up rows in
+// that is none adds nothing, with identity one from `experts` on weights x) of weights[row][choice] * down_e act(gate_e x, up_e x). up: matrices of [2 I, D], gate and up rows in
 // turn; down: matrices of [D, I].
 int64_t he_fp4_experts_workspace_bytes(int rows, int top, int experts, int I, int D);
 int he_fp4_experts(void* out, const void* x, int64_t ldx, const void* up_codes, const void* up_scales, const void* down_codes,
                    const void* down_scales, const void* ids_i32, const void* weights_f32, int rows, int top, int experts, int I, int D,
-                   int group_up, int group_down, float alpha, float limit, float up_shift, float cubic, void* workspace,
+                   int group_up, int group_down, int identity, float alpha, float limit, float up_shift, float cubic, void* workspace,
                    int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -25,7 +25,7 @@ from ..cache.paged import PagedCache
 from ..cache.pages import CacheError, CacheFull  # noqa: F401
 from ..config.base import ModelConfig, stop_token_ids
 from ..kernels import lib as kernel_lib
-from ..kernels import library_tuning, profiler
+from ..kernels import fp4, library_tuning, profiler
 from ..parts.base import BuildEnv, StepContext
 from ..registry import build_model, load_config
 from ..weights.loader import load_tensors
@@ -110,7 +110,7 @@ class Engine:
                  device: str = "cuda:0", fast_kernels: bool = True, use_graphs: bool = True,
                  tune_library: bool = False, beyond_max_positions: bool = False, profile: bool = False,
                  sync_each_launch: bool = False, graph_step_rows: int = GRAPH_MAX_STEP_ROWS,
-                 graph_chunk_rows: int = GRAPH_MAX_CHUNK_ROWS):
+                 graph_chunk_rows: int = GRAPH_MAX_CHUNK_ROWS, weights: str = "stored", weight_group: int = 64):
         """max_seq_len: the longest sequence (default: the positions the model's configuration
         allows; more than that is refused unless beyond_max_positions says it is meant).
         tune_library: let the library's autotuner choose the kernel of each tall bfloat16
@@ -122,11 +122,21 @@ class Engine:
         graph_chunk_rows: longer steps are captured as well, unpadded, when their row count is a
         multiple of 256 and at most this and they want at most 64 places (fixed prompt chunks; 0,
         or graph_step_rows 0: none).
+        weights: "stored", or "fp4": the layers' matrices are packed into 4 bits when they are loaded, in groups of `weight_group`
+        (32, 64 or 128) along K that share a scale (kernels/fp4.py), and read so by every step; bfloat16 engines only. The
+        embedding, the norms, routers and gates and the output head stay as they are stored. (The reference serves its
+        models in formats of 4 to 5 bits: tools/quant_bench/README.md:305-307.)
         sync_each_launch: a debugging mode (the reference's sync_after_each_op, src/engine.cpp:318-334):
         steps run without HIP graphs and the host waits for the GPU after every launch, so that
         a fault is reported with the name of the op that raised it."""
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be one of {sorted(_DTYPES)}, got {dtype!r}")
+        if weights not in ("stored", "fp4"):
+            raise ValueError(f"weights must be 'stored' or 'fp4', got {weights!r}")
+        if weights == "fp4" and (_DTYPES[dtype] != torch.bfloat16 or not fast_kernels):
+            raise ValueError("weights 'fp4' go with dtype 'bfloat16' and the fast kernels")
+        if weights == "fp4" and weight_group not in fp4.GROUPS:
+            raise ValueError(f"weight_group must be one of {fp4.GROUPS}, got {weight_group!r}")
         if not torch.cuda.is_available():
             raise RuntimeError("no GPU: this engine runs its HIP kernels on an MI355X only")
         kernel_lib.load()   # fails loudly when the kernel library is missing
@@ -158,6 +168,8 @@ class Engine:
             tensors = random_tensors(specs, seed, self.dtype, self.device)
         self.model.bind(tensors)
         del tensors
+        if weights == "fp4":
+            self.model.pack_weights(weight_group)
         self.vocab_size = self.model.spec.vocab_size
         allowed = self.model.spec.max_positions
         if max_seq_len is not None and max_seq_len > allowed and not beyond_max_positions:

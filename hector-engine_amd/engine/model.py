@@ -86,6 +86,14 @@ class DecoderModel:
             todo += p.children()
         self._keep_orders()
 
+    def pack_weights(self, group: int) -> None:
+        """The layers' product weights in 4 bits (kernels.fp4); embedding, norms, routers, gates and the head stay as they are."""
+        todo = list(self.parts())
+        while todo:
+            p = todo.pop()
+            p.pack_weights(group)
+            todo += p.children()
+
     def _keep_orders(self) -> None:
         """A router over rows that no norm has evened out turns near ties over at any change of a sum's order (Domorax: 4 % of its
         bfloat16 logits with another order in its one-token steps' products): where blocks hand their stream to their parts

@@ -19,17 +19,40 @@ GROUPS = (32, 64, 128)
 TILE_ROWS, TILE_K = 16, 128
 
 
+def storage_shapes(shape: tuple, group: int) -> tuple[tuple, tuple]:
+    """The shapes of the codes (uint8) and the scales (bfloat16) of a matrix [N, K], or of several [E, N, K]."""
+    if len(shape) not in (2, 3) or any(s <= 0 for s in shape):
+        raise ValueError(f"fp4: a matrix is [N, K] or [E, N, K] of positive sizes, not {tuple(shape)}")
+    if group not in GROUPS:
+        raise ValueError(f"fp4: groups of {group}, must be one of {GROUPS}")
+    *lead, n, k = shape
+    tiles = (*lead, -(-n // TILE_ROWS), -(-k // TILE_K))
+    return (*tiles, TILE_ROWS * TILE_K // 2), (*tiles, TILE_K // group, TILE_ROWS)
+
+
 class Fp4Weight:
     """A packed matrix; `shape` is the matrix's. Made by pack()."""
 
     dtype = "fp4"      # what a table of kernel routes looks it up by
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple, group: int):
-        self.codes, self.scales, self.shape, self.group = codes, scales, tuple(shape), group
+        shape = tuple(int(s) for s in shape)
+        for what, t, dtype, want in zip(("codes", "scales"), (codes, scales), (torch.uint8, torch.bfloat16), storage_shapes(shape, group)):
+            if not t.is_cuda or not t.is_contiguous() or t.device != codes.device:
+                raise ValueError(f"fp4: {what} must be contiguous tensors on one GPU")
+            if t.dtype != dtype or tuple(t.shape) != want:
+                raise ValueError(f"fp4: {what} of a matrix {shape} in groups of {group} are {dtype} {want}, not {t.dtype} {tuple(t.shape)}")
+        self._codes, self._scales, self._shape, self._group, self._index = codes, scales, shape, group, codes.get_device()
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    shape = property(lambda self: self._shape)
+    group = property(lambda self: self._group)
+    device_index = property(lambda self: self._index)
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._codes.device
 
     @property
     def nbytes(self) -> int:
@@ -44,17 +67,6 @@ class Fp4Weight:
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         ops.fp4_unpack(out, self)
         return out
-
-
-def storage_shapes(shape: tuple, group: int) -> tuple[tuple, tuple]:
-    """The shapes of the codes (uint8) and the scales (bfloat16) of a matrix [N, K], or of several [E, N, K]."""
-    if len(shape) not in (2, 3) or any(s <= 0 for s in shape):
-        raise ValueError(f"fp4: a matrix is [N, K] or [E, N, K] of positive sizes, not {tuple(shape)}")
-    if group not in GROUPS:
-        raise ValueError(f"fp4: groups of {group}, must be one of {GROUPS}")
-    *lead, n, k = shape
-    tiles = (*lead, -(-n // TILE_ROWS), -(-k // TILE_K))
-    return (*tiles, TILE_ROWS * TILE_K // 2), (*tiles, TILE_K // group, TILE_ROWS)
 
 
 def pack(w: torch.Tensor, group: int = 64) -> Fp4Weight:

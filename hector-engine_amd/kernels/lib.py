@@ -122,7 +122,7 @@ _SIGNATURES = {
     "he_fp4_product": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32,
                        c_f32, c_f32, c_ptr, c_i64, c_ptr],
     "he_fp4_experts_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
-    "he_fp4_experts": [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+    "he_fp4_experts": [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                        c_f32, c_f32, c_f32, c_f32, c_ptr, c_i64, c_ptr],
     "he_diff_heads": [c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32, c_f32, c_int, c_ptr],
     "he_attention_plain_workspace_floats": [c_int, c_int, c_int, c_int, c_int, c_int],

@@ -6,6 +6,7 @@ from __future__ import annotations
 import functools
 import torch
 
+from . import fp4 as _fp4
 from . import kv_layout as layout
 from . import lib as _lib
 from .profiler import op as _op
@@ -1393,51 +1394,44 @@ def chosen_experts(out, h_scratch, x, gate_up, down, ids, weights, dense, rows: 
                                    _stream()))
 
 
-def _fp4_here(name: str, *tensors) -> None:
-    """Tensors (None allowed) of one GPU, the current one: a launch goes to its stream."""
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name}: expected GPU tensors")
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{name}: a tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _fp4_weight(name: str, w, dims: int = 2) -> None:
-    from .fp4 import Fp4Weight, storage_shapes
-    if not isinstance(w, Fp4Weight):
+def _fp4_weight(name: str, w, dims: int) -> int:
+    """The current device, which a launch goes to and the weight has to be on (an Fp4Weight checks its own tensors when it is made)."""
+    if not isinstance(w, _fp4.Fp4Weight):
         raise TypeError(f"{name}: expected a packed weight (kernels.fp4.pack), got {type(w).__name__}")
-    codes, scales = storage_shapes(w.shape, w.group)
-    _need(w.codes, f"{name}: codes", torch.uint8, codes)
-    _need(w.scales, f"{name}: scales", torch.bfloat16, scales)
-    if w.dim() != dims:
+    if len(w.shape) != dims:
         raise ValueError(f"{name}: expected a packed weight of {dims} dims, got {w.shape}")
-    _fp4_here(name, w.codes, w.scales)
+    device = torch.cuda.current_device()
+    if w.device_index != device:
+        raise ValueError(f"{name}: a weight on cuda:{w.device_index}, the current device is cuda:{device}")
+    return device
 
 
-def _fp4_rows(name: str, t, what: str, rows: int, cols: int, dtype) -> None:
-    """[rows or more, cols] whose elements of a row are neighbours; the rows may lie apart."""
-    _fp4_here(name, t)
-    if t.dtype != dtype:
+def _fp4_on(name: str, what: str, t, device: int) -> None:
+    if t.get_device() != device:
+        raise ValueError(f"{name}: {what} is on {t.device}, expected a GPU tensor on the current device, cuda:{device}")
+
+
+def _fp4_rows(name: str, what: str, t, rows: int, cols: int, dtype, device: int) -> int:
+    """The distance of the rows of a tensor [rows or more, cols] whose elements of a row are neighbours."""
+    _fp4_on(name, what, t, device)
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: {what} is {t.dtype}, expected {dtype}")
-    if t.dim() != 2 or t.shape[1] != cols or t.shape[0] < rows:
-        raise ValueError(f"{name}: {what}{tuple(t.shape)} is not [{rows}, {cols}]")
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != cols or shape[0] < rows:
+        raise ValueError(f"{name}: {what}{tuple(shape)} is not [{rows}, {cols}]")
+    apart, step = t.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and apart < cols):
         raise ValueError(f"{name}: {what}'s rows must be contiguous and must not overlap, strides {t.stride()}")
+    return apart if rows > 1 else cols
 
 
-def _fp4_row_stride(t, cols: int) -> int:
-    return t.stride(0) if t.shape[0] > 1 else cols
-
-
-def _fp4_workspace(name: str, workspace, size: int):
+def _fp4_workspace(name: str, workspace, size: int, device: int):
     if size == 0:
         return None, 0
     if workspace is None:
         raise ValueError(f"{name}: a workspace of {size} bytes is needed")
     _need(workspace, f"{name}: workspace", torch.uint8)
-    _fp4_here(name, workspace)
+    _fp4_on(name, "workspace", workspace, device)
     if workspace.numel() < size or workspace.data_ptr() % 16:
         raise ValueError(f"{name}: a workspace of {size} bytes, 16-byte aligned, is needed; got {workspace.numel()}")
     return workspace.data_ptr(), workspace.numel()
@@ -1446,8 +1440,8 @@ def _fp4_workspace(name: str, workspace, size: int):
 @_op("fp4_pack")
 def fp4_pack(packed, w) -> None:
     """packed (kernels.fp4.Fp4Weight) = w, float32 or bfloat16, of its shape."""
-    _fp4_weight("fp4_pack", packed, packed.dim())
-    _fp4_here("fp4_pack", w)
+    device = _fp4_weight("fp4_pack", packed, len(packed.shape))
+    _fp4_on("fp4_pack", "w", w, device)
     if tuple(w.shape) != packed.shape:
         raise ValueError(f"fp4_pack: w{tuple(w.shape)} for a packed weight of {packed.shape}")
     *lead, N, K = packed.shape
@@ -1461,9 +1455,9 @@ def fp4_pack(packed, w) -> None:
 @_op("fp4_unpack")
 def fp4_unpack(out, packed) -> None:
     """out (float32 or bfloat16, contiguous) = the values of a packed weight."""
-    _fp4_weight("fp4_unpack", packed, packed.dim())
+    device = _fp4_weight("fp4_unpack", packed, len(packed.shape))
     _need(out, "fp4_unpack: out", shape=packed.shape)
-    _fp4_here("fp4_unpack", out)
+    _fp4_on("fp4_unpack", "out", out, device)
     *lead, N, K = packed.shape
     _lib.check(_lib.load().he_fp4_unpack(out.data_ptr(), packed.codes.data_ptr(), packed.scales.data_ptr(), lead[0] if lead else 1, N, K,
                                          packed.group, dtype_code(out.dtype), _stream()))
@@ -1480,27 +1474,26 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.
     or, gated, out[rows, N / 2] (bfloat16, no bias) = act(gate, up) for a weight that alternates gate and up rows, act =
     (alpha, limit, up_shift[, cubic]) the activation's constants as silu_mul takes them. The rows of x and out may lie apart.
     workspace: uint8, fp4_product_workspace_bytes(rows, w, gated) or more; calls that may run at the same time need one each."""
-    _fp4_weight("fp4_product", w)
+    device = _fp4_weight("fp4_product", w, 2)
     N, K = w.shape
     if rows < 0:
         raise ValueError(f"fp4_product: {rows} rows")
     if gated and (N % 2 or bias is not None):
         raise ValueError("fp4_product: a gated product has an even number of weight rows and no bias")
-    _fp4_rows("fp4_product", x, "x", rows, K, torch.bfloat16)
-    if out.dtype not in ((torch.bfloat16,) if gated else (torch.bfloat16, torch.float32)):
-        raise TypeError(f"fp4_product: results in {out.dtype}")
-    cols = N // 2 if gated else N
-    _fp4_rows("fp4_product", out, "out", rows, cols, out.dtype)
+    ldx = _fp4_rows("fp4_product", "x", x, rows, K, torch.bfloat16, device)
+    dtype = out.dtype
+    if dtype is not torch.bfloat16 and (gated or dtype is not torch.float32):
+        raise TypeError(f"fp4_product: results in {dtype}")
+    ldo = _fp4_rows("fp4_product", "out", out, rows, N // 2 if gated else N, dtype, device)
     if bias is not None:
         _need(bias, "fp4_product: bias", shape=(N,))
-        _fp4_here("fp4_product", bias)
-    ws, size = _fp4_workspace("fp4_product", workspace, fp4_product_workspace_bytes(rows, w, gated))
+        _fp4_on("fp4_product", "bias", bias, device)
+    L = _lib.load()
+    ws, size = _fp4_workspace("fp4_product", workspace, L.he_fp4_product_workspace_bytes(rows, N, K, gated), device)
     if rows == 0:
         return
-    _lib.check(_lib.load().he_fp4_product(
-        out.data_ptr(), _fp4_row_stride(out, cols), x.data_ptr(), _fp4_row_stride(x, K), w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), rows,
-        N, K, w.group, dtype_code(out.dtype), dtype_code(bias.dtype) if bias is not None else F32, int(gated), *_act4(act), ws, size,
-        _stream()))
+    _lib.check(L.he_fp4_product(out.data_ptr(), ldo, x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), rows, N, K, w.group,
+                                dtype_code(dtype), F32 if bias is None else dtype_code(bias.dtype), gated, *_act4(act), ws, size, _stream()))
 
 
 def fp4_experts_workspace_bytes(rows: int, top: int, gate_up, down) -> int:
@@ -1510,35 +1503,36 @@ def fp4_experts_workspace_bytes(rows: int, top: int, gate_up, down) -> int:
 
 
 @_op("fp4_experts")
-def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0, 0.0), workspace=None) -> None:
+def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0, 0.0), identity: bool = False, workspace=None) -> None:
     """A routed feed-forward over packed experts: out[rows, D] (bfloat16) = the sum over a row's choices c of weights[row, c] *
-    down[e] act(gate[e] x, up[e] x) with e = ids[row, c]; an id that is no expert adds nothing, nor does a weight of 0. gate_up: packed
-    [E, 2 I, D], gate i of an expert in row 2 i, its up in 2 i + 1; down: packed [E, D, I]; ids int32, weights float32
+    down[e] act(gate[e] x, up[e] x) with e = ids[row, c]; an id that is no expert adds nothing, nor does a weight of 0; with identity an id from E on adds
+    weights[row, c] * x. gate_up: packed [E, 2 I, D], gate i of an expert in row 2 i, its up in 2 i + 1; down: packed [E, D, I]; ids int32, weights float32
     [rows, top]; x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. workspace: uint8,
     fp4_experts_workspace_bytes(rows, top, gate_up, down) or more; calls that may run at the same time need one each."""
-    _fp4_weight("fp4_experts", gate_up, 3)
+    device = _fp4_weight("fp4_experts", gate_up, 3)
     _fp4_weight("fp4_experts", down, 3)
     E, D, I = down.shape
     if gate_up.shape != (E, 2 * I, D):
         raise ValueError(f"fp4_experts: gate_up{gate_up.shape} for down{down.shape}, expected {(E, 2 * I, D)}")
     if rows < 0:
         raise ValueError(f"fp4_experts: {rows} rows")
-    _fp4_rows("fp4_experts", x, "x", rows, D, torch.bfloat16)
+    ldx = _fp4_rows("fp4_experts", "x", x, rows, D, torch.bfloat16, device)
     _need(out, "fp4_experts: out", torch.bfloat16)
-    _fp4_rows("fp4_experts", out, "out", rows, D, torch.bfloat16)
+    _fp4_rows("fp4_experts", "out", out, rows, D, torch.bfloat16, device)
     _need(ids, "fp4_experts: ids", torch.int32)
     _need(weights, "fp4_experts: weights", torch.float32)
-    _fp4_here("fp4_experts", ids, weights)
+    _fp4_on("fp4_experts", "ids", ids, device)
+    _fp4_on("fp4_experts", "weights", weights, device)
     if ids.dim() != 2 or ids.shape[0] < rows or ids.shape[1] == 0 or weights.shape != ids.shape:
         raise ValueError(f"fp4_experts: ids{tuple(ids.shape)} and weights{tuple(weights.shape)} are not [{rows}, choices]")
     top = ids.shape[1]
-    ws, size = _fp4_workspace("fp4_experts", workspace, fp4_experts_workspace_bytes(rows, top, gate_up, down))
+    L = _lib.load()
+    ws, size = _fp4_workspace("fp4_experts", workspace, L.he_fp4_experts_workspace_bytes(rows, top, E, I, D), device)
     if rows == 0:
         return
-    _lib.check(_lib.load().he_fp4_experts(
-        out.data_ptr(), x.data_ptr(), _fp4_row_stride(x, D), gate_up.codes.data_ptr(), gate_up.scales.data_ptr(), down.codes.data_ptr(),
-        down.scales.data_ptr(), ids.data_ptr(), weights.data_ptr(), rows, top, E, I, D, gate_up.group, down.group, *_act4(act), ws, size,
-        _stream()))
+    _lib.check(L.he_fp4_experts(out.data_ptr(), x.data_ptr(), ldx, gate_up.codes.data_ptr(), gate_up.scales.data_ptr(), down.codes.data_ptr(),
+                                down.scales.data_ptr(), ids.data_ptr(), weights.data_ptr(), rows, top, E, I, D, gate_up.group, down.group,
+                                identity, *_act4(act), ws, size, _stream()))
 
 
 @_op("diff_heads")

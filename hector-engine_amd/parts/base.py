@@ -240,6 +240,14 @@ class Part:
     def children(self) -> list["Part"]:
         return []
 
+    def pack_weights(self, group: int) -> None:
+        """Its products' weights in 4 bits from here on (kernels.fp4), in groups of `group` along K; called once, after bind().
+        The layers that a part holds as attributes are packed for it: a part overrides this for weights it keeps otherwise."""
+        from .linear import Linear
+        for lin in vars(self).values():
+            if isinstance(lin, Linear):
+                lin.pack(group)
+
     def step_columns(self) -> int:
         """Columns (activation dtype) of rows this part wants to keep until the step's end, beyond its layer's turn:
         the model then gives it ctx.room[self], [rows, columns], in every step. 0: none."""

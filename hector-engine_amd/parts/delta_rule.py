@@ -98,6 +98,7 @@ class GatedDeltaRule(Mixer):
         # the gates' rows stay in the stored dtype: the products are exact in 32 bits, and the sums and the result
         # are 32-bit (out_dtype below)
         self.gates = Linear(torch.cat([tensors[n["b"]], tensors[n["a"]]], 0).contiguous())
+        self.gates.packable = False         # (a few rows, and they steer the memory)
         self.taps = torch.cat([tensors[n[x]] for x in ("q_conv", "k_conv", "v_conv")], 0).contiguous()
         self.a_log, self.dt_bias = tensors[n["A_log"]], tensors[n["dt_bias"]]
         if self.a_log.dtype != self.dt_bias.dtype:

@@ -73,6 +73,7 @@ class LinearHead(Part):
     def bind(self, tensors):
         name = self.tied_to or self._name
         self.linear = Linear(tensors[name])
+        self.linear.packable = False        # (the logits of a step come from the matrix as it is stored)
 
     def forward(self, x: torch.Tensor, rows: int, ctx: StepContext) -> torch.Tensor:
         return self.linear(x, rows, ctx, out_dtype=torch.float32)

@@ -18,6 +18,8 @@ registers:
                               (_long, tall_gated, gated_tile, _few_tiles)
   fp32 results (logits)    -> the MFMA kernels up to 64 rows, above that the library,
                               which writes fp32 from bf16 operands
+  packed weights (4 bits)  -> the kernels that read them (kernels.fp4), any number of rows; the gated
+                              activation is their epilogue at any number too
 
 Both MFMA kernels carry an RMS norm across a pair of products, so that a step of up to 64
 rows has no norm kernels: given a :class:`ResidualSink` the product adds its result
@@ -37,7 +39,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ..kernels import library_tuning, ops, profiler, routes
+from ..kernels import fp4, library_tuning, ops, profiler, routes
 from .base import NormedRows, PieceRows, ResidualSink, StepContext
 
 BF16, F32 = torch.bfloat16, torch.float32
@@ -70,10 +72,18 @@ class Linear:
         self.bias = bias
         self.out_features, self.in_features = weight.shape
         self.one_round_tiles = False        # set by a part: _long's, gated_tile's and K slices' products may run in tiles of this library's own
+        self.packable = True                # set by a part: pack() may take the weight
         self.ordered = False                # set by the model: the few-rows product keeps an older order of sums (ops.gemm_blocksplit)
         self._plans: dict[bool, tuple[int, int]] = {}
         self._chosen: dict[tuple, routes.Route] = {}     # (rows, activations, fast) -> route, for one version of the table
         self._chosen_version = -1
+
+    def pack(self, group: int) -> None:
+        """The weight in 4 bits from here on (kernels.fp4), where the part allows it; the stored one is let go."""
+        if self.packable and not isinstance(self.weight, fp4.Fp4Weight):
+            self.weight = fp4.pack(self.weight, group)
+            self._plans.clear()
+            self._chosen.clear()
 
     def route(self, rows: int, ctx: StepContext, act: torch.dtype) -> routes.Route:
         """The kernel route of this product at this many rows of this activation dtype (remembered
@@ -197,6 +207,15 @@ class Linear:
         if y32 is not out:
             out[:rows].copy_(y32)
         return out
+
+    def _run_fp4(self, x, rows, ctx, bias, out_dtype, out, sink):
+        x, out = self._dense(x, rows, ctx, out_dtype, out)
+        self._fp4(out, x, bias, rows, ctx)
+        return out
+
+    def _fp4(self, out, x, bias, rows: int, ctx: StepContext, **epilogue) -> None:
+        size = ops.fp4_product_workspace_bytes(rows, self.weight, bool(epilogue))
+        ops.fp4_product(out, x, self.weight, bias, rows, workspace=ctx.scratch.transient((size,), torch.uint8) if size else None, **epilogue)
 
     def _run_library(self, x, rows, ctx, bias, out_dtype, out, sink):
         x, out = self._dense(x, rows, ctx, out_dtype, out)
@@ -374,6 +393,11 @@ class Linear:
         act_dtype, a, scale, pieces = _operand(x)
         if not self.gated_silu_rows(rows, ctx, act_dtype):
             raise ValueError("Linear.gated_silu: not for these rows (ask gated_silu_rows)")
+        if isinstance(self.weight, fp4.Fp4Weight):
+            if out_pieces:
+                raise ValueError("Linear.gated_silu: a packed weight's product writes row-major (ask gated_pieces)")
+            self._fp4(out, x.tensor(ctx) if isinstance(x, NormedRows) else a, None, rows, ctx, gated=True, act=consts)
+            return
         if rows <= ops.BLOCKSPLIT_PIECES_MAX_M:
             ops.gemm_blocksplit(out, a, self.weight, None, rows, gated=True, row_scale=scale,
                                 x_pieces=pieces, out_pieces=out_pieces, act=consts, ordered=self.ordered)
@@ -403,7 +427,7 @@ class Linear:
         9728 x 896 at 768 rows 22.5 beside 24.9, at 1400 36.4 beside 36.8; 29824 x 704 at 149 rows 1.21). With fewer tiles units idle (1024 x 256 at
         1000 rows 12.7, 8.0)."""
         N, K = self.weight.shape
-        if not (K <= 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0 and N % 8 == 0
+        if isinstance(self.weight, fp4.Fp4Weight) or not (K <= 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0 and N % 8 == 0
                 and ops.tiles_read(x, self.weight) and self.own_tiles(rows, ctx)) or library_tuning.enabled():
             return 0             # (a tuned choice of the library has not been measured against)
         if self._rounds(rows, 128) <= 1:
@@ -419,7 +443,7 @@ class Linear:
         beside 85, 100 rows 58 beside 71); with several rows of tiles and less of them real 0.77 to 1.24 (259 x 28672 x 4096 100 us, the two 82,
         541 x 37888 x 2048 106 and 98), with tiles for less than 0.8 of the rounds up to 1.48. Only where a part allows it (one_round_tiles): see _long."""
         N, K = self.weight.shape
-        if not (self.one_round_tiles and K > 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0
+        if isinstance(self.weight, fp4.Fp4Weight) or not (self.one_round_tiles and K > 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0
                 and N % 8 == 0 and self.weight.is_contiguous() and ops.tiles_read(x, self.weight) and self.own_tiles(rows, ctx)) \
                 or library_tuning.enabled():
             return None
@@ -445,6 +469,8 @@ class Linear:
 
     def gated_pieces(self, rows: int) -> bool:
         """Whether gated_silu can write its result piece-major at this many rows."""
+        if isinstance(self.weight, fp4.Fp4Weight):
+            return False
         return rows <= ops.BLOCKSPLIT_PIECES_MAX_M or self._plan(rows)[1] == 1
 
 
@@ -457,5 +483,6 @@ routes.register_route("linear", (BF16, BF16), "mfma", _mfma_takes, Linear._run_m
                       traits=("pieces", "gated", "k_slices"))
 routes.register_route("linear", (BF16, BF16), "plain", lambda c: not c.fast or c.K % 8 != 0, Linear._run_plain)
 routes.register_route("linear", (BF16, BF16), "library", lambda c: True, Linear._run_library)
+routes.register_route("linear", (fp4.Fp4Weight.dtype, BF16), "fp4", lambda c: True, Linear._run_fp4, traits=("gated",))
 routes.register_route("linear", (F32, F32), "plain", lambda c: True, Linear._run_plain)
 routes.register_route("linear", (F32, BF16), "plain_widened", lambda c: True, Linear._run_plain_widened)

@@ -85,6 +85,7 @@ class MatrixMemory(Mixer):
         # the gates' rows stay in the stored dtype: products of bfloat16 numbers are exact in 32 bits, and the sums
         # and the result are 32-bit (out_dtype below), so nothing that enters the exponentials is rounded to 16 bits
         self.gates = Linear(torch.cat([tensors[n["i"]], tensors[n["f"]]], 0).contiguous())
+        self.gates.packable = False         # (a few rows, and they steer the memory)
         self.gate_bias = torch.cat([tensors[n["i_bias"]].to(f32), tensors[n["f_bias"]].to(f32)], 0).contiguous()
         self.o_proj = Linear(tensors[n["o"]])
         self.norm = tensors[n["norm"]]

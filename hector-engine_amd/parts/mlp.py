@@ -79,6 +79,9 @@ class GatedMLP(FeedForward):
 
     def _gate(self, h, x, rows: int, ctx: StepContext) -> None:
         """h[rows, inter] = act(gate x, up x) of many rows: one kernel where the product takes the activation along."""
+        if self.gate_up.gated_silu_rows(rows, ctx, x.scaled.dtype if isinstance(x, NormedRows) else x.dtype):
+            self.gate_up.gated_silu(x, rows, ctx, h, act=self.act)
+            return
         if isinstance(x, NormedRows) and self.gate_up.own_tiles(rows, ctx, x.scaled.dtype):
             x = x.tensor(ctx)
         bm = self.gate_up.tall_gated(rows, ctx, x)

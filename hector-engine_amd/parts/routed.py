@@ -27,13 +27,15 @@ suffix of its prefix, "gate": suffix of a stored vector of hidden_size or None} 
 uses, out += sigmoid(gate . n) * shared(n) (gate None: out += shared(n)), the dot product in fp32; `router_bias` adds a
 stored number an output to the logits. A shared expert without a gate whose activation is the experts' own joins their
 fused matrices as columns of weight 1: it costs no launch of its own.
+Packed (pack_weights): each expert's matrices in 4 bits, one operator for all of them and any number of rows (ops.fp4_experts); a shared
+expert's columns are then a feed-forward of their own beside it.
 names: the suffixes of its tensors (router, router_bias, correction; expert e's are 'e<e>.' + gate / up / down).
 """
 from __future__ import annotations
 
 import torch
 
-from ..kernels import ops
+from ..kernels import fp4, ops
 from .base import BuildEnv, FeedForward, NormedRows, PartSpec, StepContext, TensorSpec, build_part, param, register_part, tensor_name
 from .linear import Linear
 from .mlp import GatedMLP
@@ -103,6 +105,7 @@ class RoutedExperts(FeedForward):
         self.correction = None
         self.gate_up: Linear | None = None
         self.down: Linear | None = None
+        self.packed = None                  # (gate||up and down of the experts; of the shared columns or None), packed
 
     def _name(self, e: int, which: str) -> str:
         return self.prefix + self._expert.format(e=e) + self._sub[which]
@@ -152,6 +155,41 @@ class RoutedExperts(FeedForward):
                 lin.one_round_tiles = False                # (the router may read rows no norm has evened out)
         if self._shared_gate:
             self.shared_gate = tensors[self._shared_gate].reshape(-1).contiguous()
+
+    def pack_weights(self, group: int) -> None:
+        E, I, S, D = self.real, self.inter, self.shared_cols, self.hidden
+        up, down = self.gate_up.weight, self.down.weight
+        experts = (fp4.pack(up[:2 * E * I].view(E, 2 * I, D), group),
+                   fp4.pack(down[:, :E * I].view(D, E, I).transpose(0, 1).contiguous(), group))
+        shared = None
+        if S:
+            shared = Linear(up[2 * E * I:2 * (E * I + S)]), Linear(down[:, E * I:E * I + S].contiguous())
+            for lin in shared:
+                lin.pack(group)
+        self.packed = (*experts, shared)
+        self.gate_up = self.down = None
+
+    def _packed_experts(self, x, ids, weights, ctx: StepContext):
+        up, down, shared = self.packed
+        rows, act = ctx.rows, (self.alpha, self.limit, self.up_shift)
+        out = ctx.alloc((rows, self.hidden))
+        for r0 in range(0, rows, _ROW_CHUNK):
+            n = min(_ROW_CHUNK, rows - r0)
+            size = ops.fp4_experts_workspace_bytes(n, self.top, up, down)
+            ops.fp4_experts(out[r0:r0 + n], x[r0:r0 + n], up, down, ids[r0:r0 + n], weights[r0:r0 + n], n, act=act,
+                            identity=self.identity > 0, workspace=ctx.scratch.transient((size,), torch.uint8))
+        if shared is None:
+            return out
+        both = ctx.alloc((rows, self.hidden))
+        for r0 in range(0, rows, _ROW_CHUNK):
+            n = min(_ROW_CHUNK, rows - r0)
+            turn = ctx.scratch.mark()
+            h = ctx.alloc((n, self.shared_cols))
+            shared[0].gated_silu(x[r0:r0 + n], n, ctx, h, act={"alpha": self.alpha, "limit": self.limit, "up_shift": self.up_shift})
+            common = shared[1](h, n, ctx)
+            ops.scaled_sum(both[r0:r0 + n], out[r0:r0 + n], common, n, 1.0, 1.0)
+            ctx.scratch.release(turn)
+        return both
 
     def _few_rows(self, rows: int, x, ctx: StepContext) -> bool:
         """Whether the step runs through the chosen experts alone (kernels.ops.chosen_experts): bfloat16 with the
@@ -258,6 +296,8 @@ class RoutedExperts(FeedForward):
 
     def _routed(self, x, ctx: StepContext, may_sink: bool):
         rows, real, I, S = ctx.rows, self.real, self.inter, self.shared_cols
+        if self.packed is not None and isinstance(x, NormedRows):
+            x = x.tensor(ctx)
         # rows a product has left for this norm: read as they lie where they owe nothing (and no identity expert wants
         # them row by row), else made into a tensor, by the router's launch where that pays and its reads are whole
         pieces = isinstance(x, NormedRows) and x.finished and x.pieces and not self.identity
@@ -281,6 +321,8 @@ class RoutedExperts(FeedForward):
         ops.route_tokens(dense, ids, weights, None, self.correction, rows, real, self.groups, self.keep,
                          self.top, self.scale, x=read, router=self.router, normalize=self.normalize, bias=self.bias,
                          x_pieces=read_pieces, owed=owed)
+        if self.packed is not None:
+            return self._packed_experts(x, ids, weights, ctx)
         cols = real * I + S + (self.hidden if self.identity else 0)
         act = {"alpha": self.alpha, "limit": self.limit, "up_shift": self.up_shift}
         if self._few_rows(rows, x, ctx):
