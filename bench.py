@@ -75,10 +75,14 @@ FP32_PEAK_FLOPS = 157.3e12
 LONG_PROMPT = 7800   # the long-context point: prompts of so many tokens in the shape's context
 
 
-def weight_bytes(c, layers, itemsize=2):
+def weight_bytes(c, layers, itemsize=2, group=0):
+    """group: the layers' matrices in 4 bits, so many neighbours sharing a scale of 16."""
     D, H, KVH, hd, I, V = (c["hidden_size"], c["num_attention_heads"], c["num_key_value_heads"],
                            c["head_dim"], c["intermediate_size"], c["vocab_size"])
     per_layer = D * (H + 2 * KVH) * hd + (H + 2 * KVH) * hd + H * hd * D + 3 * D * I + 2 * D
+    if group:
+        matrices = D * (H + 2 * KVH) * hd + H * hd * D + 3 * D * I
+        return itemsize * (layers * (per_layer - matrices) + D + V * D) + layers * matrices * (0.5 + 2 / group)
     return itemsize * (layers * per_layer + D + V * D)      # lm_head read once; embedding rows are negligible
 
 
@@ -353,6 +357,9 @@ def main() -> int:
                          "the sampling presets; reported as \"generation\", decoded tokens a second")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16",
                     help="float32: the whole measurement in true 32-bit (no library products, no extra points)")
+    ap.add_argument("--weights", choices=["stored", "fp4"], default="stored",
+                    help="fp4: the layers' matrices packed into 4 bits (no extra points)")
+    ap.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=64)
     ap.add_argument("--no-tune", action="store_true",
                     help="leave the library's default kernels for the tall matrix products")
     ap.add_argument("--design-sizes", default="", help=f"with --design: only these of {', '.join(DESIGN_SIZES)}")
@@ -406,17 +413,18 @@ def main() -> int:
     class Model:
         """An engine of one shape and precision with what the measurements need of it."""
 
-        def __init__(self, shape, layers, dtype, max_batch, context, tune):
+        def __init__(self, shape, layers, dtype, max_batch, context, tune, packing=None):
+            packing = packing or {}
             self.shape, self.layers, self.context = shape, layers, context
             self.itemsize = 2 if dtype == "bfloat16" else 4
             config = Qwen2Config.from_dict(dict(shape, num_hidden_layers=layers, architectures=["Qwen2ForCausalLM"]))
             t0 = time.perf_counter()
             self.engine = he.Engine(config=config, seed=0, dtype=dtype, max_tokens=max_batch * context,
-                                    max_slots=max_batch, max_seq_len=context, tune_library=tune)
+                                    max_slots=max_batch, max_seq_len=context, tune_library=tune, **packing)
             self.sampler = he.Sampler(he.SamplingConfig.deterministic(), self.engine.device)
             torch.cuda.synchronize()
             self.load_s = time.perf_counter() - t0
-            self.wbytes = weight_bytes(shape, layers, self.itemsize)
+            self.wbytes = weight_bytes(shape, layers, self.itemsize, packing.get("weight_group", 0))
             self.packed = {}
 
         def prompts(self, n, lo, hi):
@@ -526,7 +534,8 @@ def main() -> int:
     fp32 = args.dtype == "float32"
     if fp32:
         args.no_tune = True
-    model = Model(SHAPE, args.layers, args.dtype, max_batch, CONTEXT, not args.no_tune)
+    packing = {"weights": "fp4", "weight_group": args.weight_group} if args.weights == "fp4" else None
+    model = Model(SHAPE, args.layers, args.dtype, max_batch, CONTEXT, not args.no_tune, packing)
     engine, load_s = model.engine, model.load_s
 
     # ---- prefill of one 2,048-token prompt
@@ -629,7 +638,7 @@ def main() -> int:
                 decode_ms = max(r.decode_ms for r in results)
                 tokens = sum(len(r.tokens) for r in results)
                 generation[f"b{b}_{name}"] = round((tokens - b) * 1e3 / decode_ms, 1)
-    extra = not args.no_extra and not args.no_points and args.shape == "7b" and args.layers == FULL_LAYERS and not fp32
+    extra = not args.no_extra and not args.no_points and args.shape == "7b" and args.layers == FULL_LAYERS and not fp32 and not packing
     prefill_fp32 = None
     if extra:
         # the large batch behind long prompts: 32 steps a run keep the sequences inside the context
@@ -652,7 +661,7 @@ def main() -> int:
 
     PROMPTS = PROMPT_LO if PROMPT_LO == PROMPT_HI else f"{PROMPT_LO}-{PROMPT_HI}"
     line = {
-        "metric": f"decode tok/s @ bs {args.batch}, {MODEL} {'fp32' if fp32 else 'bf16'}, context {CONTEXT}, prompts {PROMPTS}",
+        "metric": f"decode tok/s @ bs {args.batch}, {MODEL} {'fp32' if fp32 else 'bf16'}{f', 4-bit weights in groups of {args.weight_group}' if packing else ''}, context {CONTEXT}, prompts {PROMPTS}",
         "value": round(args.batch / step_s, 1),
         "unit": "tokens/s",
         "n_gpus": 1,
