@@ -54,7 +54,7 @@ struct Fp4Case {
   bool out_f32, gated;
   const void* bias;           // [N] or null
   int bias_dtype;
-  int M;
+  int M;                      // with groups: the most slots that a group can have
   GatedAct act;
   const int32_t* tile_begin;  // [groups + 1]: a group's first tile of slots; null: no groups
   int groups;
@@ -126,7 +126,7 @@ __device__ __forceinline__ int fp4_group_of(const int32_t* tile_begin, int group
   return lo;
 }
 
-// fp4_few.hip: rows in tiles of 16
+// fp4_few.hip: rows in tiles of 16, of which the first M are real
 int fp4_run_few(const Fp4Case& c, int mtiles, hipStream_t s);
 // fp4_tall.hip: rows in tiles of 16 mt, mtiles of them at most, weight rows in tiles of 64 nt; x may be read 16 bytes at a time, K is a multiple of
 // 128. slices > 1: K cut in so many (of a block at least), their sums by way of parts [slices][M][N rounded up to 16].

@@ -3,11 +3,14 @@
 
 namespace {
 
-// A workgroup has NT tiles of 16 weight rows; its W wavefronts cut K among them, and their sums meet in LDS. A wavefront's codes, scales and
-// operands of X come straight from memory, D blocks of 128 k ahead, with no barrier before the end.
-template <int NT, int W, int D, int GROUPS, bool WHOLE>
+// A workgroup has NT tiles of 16 weight rows; its W wavefronts cut K among them, and their sums meet in LDS. Codes, scales and X (4 XL rows of it)
+// come straight into registers, D blocks of 128 k ahead, with no barrier before the end. A block of X goes from there through a
+// wavefront's own part of LDS into the order of the operands: read as operands from memory, each of its rows a sixteen-byte piece a
+// lane and all 16 of them whatever X has, it took a third of the time (8 rows of 37888 x 3584 19.5 us, without it 14).
+// There the pieces of a row lie at their index xor the row, so that the rows of an operand are in different banks.
+template <int NT, int W, int D, int XL, int GROUPS, bool WHOLE>
 __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[W * NT * 1024];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[W * (NT > 2 * XL ? NT : 2 * XL) * 1024];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
   const int blocks = c.w.blocks, lo = blocks * wave / W, hi = blocks * (wave + 1) / W;
   int group = 0;
@@ -24,11 +27,17 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     codes[j] = c.w.codes + at * FP4_TILE_BYTES;
     scales[j] = c.w.scales + at * (16 * GROUPS);
   }
-  // (an operand's rows behind the last repeat it: each row's results are its own)
-  const uint16_t* x = c.x + (c.rows_of ? (int64_t)max(c.rows_of[m0 + r16], 0) : min(m0 + r16, c.M - 1)) * c.ldx;
+  // a lane's pieces of X: row 4 i + (lane >> 4), eight k from 8 (lane & 15) on (rows behind the last repeat it: each row's results are its own)
+  const uint16_t* x[XL];
+#pragma unroll
+  for (int i = 0; i < XL; ++i) {
+    const int slot = m0 + 4 * i + kq;
+    x[i] = c.x + (c.rows_of ? (int64_t)max(c.rows_of[slot], 0) : min(slot, c.M - 1)) * c.ldx;
+  }
   const int K = c.w.K;
+  uint8_t* own = lds + wave * (2 * XL * 1024);
 
-  uint4 q[D][NT], xs[D][4];
+  uint4 q[D][NT], xs[D][XL];
   uint2 s[D][NT][GROUPS];
   auto load = [&](int u, int kb) {
 #pragma unroll
@@ -37,28 +46,38 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) s[u][j][g] = *reinterpret_cast<const uint2*>(scales[j] + (int64_t)kb * (16 * GROUPS) + 16 * g + 4 * kq);
     }
+    const int k = kb * FP4_K + 8 * r16;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int k = kb * FP4_K + 32 * t + 8 * kq;
+    for (int i = 0; i < XL; ++i) {
       if (WHOLE) {
-        xs[u][t] = *reinterpret_cast<const uint4*>(x + min(k, K - 8));
+        xs[u][i] = *reinterpret_cast<const uint4*>(x[i] + min(k, K - 8));
       } else {
         uint32_t words[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (k + e < K) words[e >> 1] |= (uint32_t)x[k + e] << (16 * (e & 1));
-        xs[u][t] = make_uint4(words[0], words[1], words[2], words[3]);
+          if (k + e < K) words[e >> 1] |= (uint32_t)x[i][k + e] << (16 * (e & 1));
+        xs[u][i] = make_uint4(words[0], words[1], words[2], words[3]);
       }
     }
   };
+  // X of a block into one of two places
+  auto keep = [&](int u, int kb, int place) {
+    const bool behind = WHOLE && kb * FP4_K + 8 * r16 >= K;
+#pragma unroll
+    for (int i = 0; i < XL; ++i) {
+      const int row = 4 * i + kq;
+      *reinterpret_cast<uint4*>(own + place * (XL * 1024) + row * 256 + (r16 ^ row) * 16) = behind ? make_uint4(0, 0, 0, 0) : xs[u][i];
+    }
+  };
+  const int xrow = min(r16, 4 * XL - 1);
   fp4_f32x4 acc[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j] = fp4_f32x4{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](int u, int kb) {
-    if (WHOLE && (kb + 1) * FP4_K > K)
+  auto multiply = [&](int u, int place) {
+    fp4_bf16x8 v[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (kb * FP4_K + 32 * t + 8 * kq >= K) xs[u][t] = make_uint4(0, 0, 0, 0);
+    for (int t = 0; t < 4; ++t)
+      v[t] = *reinterpret_cast<const fp4_bf16x8*>(own + place * (XL * 1024) + xrow * 256 + ((4 * t + kq) ^ xrow) * 16);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const uint32_t words[4] = {q[u][j].x, q[u][j].y, q[u][j].z, q[u][j].w};
@@ -66,7 +85,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const fp4_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_operand(words[t]), __builtin_bit_cast(fp4_bf16x8, xs[u][t]),
+        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_operand(words[t]), v[t],
                                                        t % (4 / GROUPS) == 0 ? zero : part, 0, 0, 0);
         if ((t + 1) % (4 / GROUPS) == 0) {
           const uint2 b = s[u][j][t / (4 / GROUPS)];
@@ -84,14 +103,19 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     for (; kb + D < hi; kb += D) {
 #pragma unroll
       for (int u = 0; u < D; ++u) {
-        multiply(u, kb + u);
+        keep(u, kb + u, u & 1);
+        multiply(u, u & 1);
         load(u, min(kb + D + u, hi - 1));
       }
     }
 #pragma unroll
     for (int u = 0; u < D; ++u)
-      if (kb + u < hi) multiply(u, kb + u);
+      if (kb + u < hi) {
+        keep(u, kb + u, u & 1);
+        multiply(u, u & 1);
+      }
   }
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < NT; ++j) *reinterpret_cast<fp4_f32x4*>(lds + (wave * NT + j) * 1024 + lane * 16) = acc[j];
   __syncthreads();
@@ -110,24 +134,35 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   }
 }
 
-template <int NT, int W, int D, bool WHOLE>
+template <int NT, int W, int D, int XL, bool WHOLE>
 int run_few(const Fp4Case& c, int mtiles, hipStream_t s) {
   const dim3 grid((c.w.tiles + NT - 1) / NT, mtiles);
-  if (c.w.group == 128) fp4_few_kernel<NT, W, D, 1, WHOLE><<<grid, 64 * W, 0, s>>>(c);
-  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, 2, WHOLE><<<grid, 64 * W, 0, s>>>(c);
-  else fp4_few_kernel<NT, W, D, 4, WHOLE><<<grid, 64 * W, 0, s>>>(c);
+  if (c.w.group == 128) fp4_few_kernel<NT, W, D, XL, 1, WHOLE><<<grid, 64 * W, 0, s>>>(c);
+  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, XL, 2, WHOLE><<<grid, 64 * W, 0, s>>>(c);
+  else fp4_few_kernel<NT, W, D, XL, 4, WHOLE><<<grid, 64 * W, 0, s>>>(c);
   return he_check_launch("he_fp4_product");
+}
+
+template <int XL>
+int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
+  if (!c.whole || c.w.K % 8) return run_few<1, 8, 2, XL, false>(c, mtiles, s);
+  // Microseconds of (tiles, wavefronts, blocks ahead) = (1, 8, 2), (1, 8, 4), (2, 4, 2), (2, 8, 2), (4, 4, 2), weights from memory:
+  // 1 row of 4608 x 3584 5.0, 5.4, 5.5, 4.8, 7.0; 3584 x 18944 10.5, 9.3, 17.4, 12.4, 23.8; 5120 x 27648 19.8, 20.2, 25.0, 17.6, 33.5; 8 rows of
+  // 37888 x 3584 21.2, 23.3, 17.3, 17.6, 18.4; 16 rows of 10240 x 5120 15.3, 20.0, 12.9, 14.0, 10.7, of 3584 x 18944 16.4, 17.1, 20.5, 20.0, 26.5.
+  const int64_t tiles = (int64_t)c.w.tiles * mtiles;
+  if (tiles <= 256) {
+    if constexpr (XL == 1) {
+      if (c.w.blocks >= 64) return run_few<1, 8, 4, XL, true>(c, mtiles, s);
+    }
+    return run_few<1, 8, 2, XL, true>(c, mtiles, s);
+  }
+  if (XL == 4 && tiles >= 640) return run_few<4, 4, 2, XL, true>(c, mtiles, s);
+  return tiles <= 512 && c.w.blocks >= 64 ? run_few<2, 8, 2, XL, true>(c, mtiles, s) : run_few<2, 4, 2, XL, true>(c, mtiles, s);
 }
 
 }  // namespace
 
 int fp4_run_few(const Fp4Case& c, int mtiles, hipStream_t s) {
   HE_REQUIRE(mtiles <= 65535, "he_fp4_product: %d tiles of rows are too many for one launch", mtiles);
-  if (!c.whole || c.w.K % 8) return run_few<1, 8, 2, false>(c, mtiles, s);
-  // The fewest tiles a workgroup that leave enough workgroups: X is read once a workgroup. Microseconds of 1 tile of 8 wavefronts, 2 of 4, 4 of 4:
-  // 1 row of 4608 x 3584 6.7, 5.7, 8.1; 3584 x 18944 14.0, 16.9, 26.9; 5120 x 27648 31.1, 23.7, 37.7; 8 rows of 37888 x 3584 31.9, 22.9, 21.5.
-  const int64_t tiles = (int64_t)c.w.tiles * mtiles;
-  if (tiles >= 2048) return run_few<4, 4, 2, true>(c, mtiles, s);
-  if (tiles >= 256 || c.w.blocks <= 32) return run_few<2, 4, 2, true>(c, mtiles, s);
-  return run_few<1, 8, 2, true>(c, mtiles, s);
+  return c.M > 8 ? run_rows<4>(c, mtiles, s) : c.M > 4 ? run_rows<2>(c, mtiles, s) : run_rows<1>(c, mtiles, s);
 }

@@ -1,4 +1,5 @@
 // Products with a weight in 4 bits (fp4.h): out[m][n] = sum_k X[m][k] W[n][k], the rows X bf16, sums 32-bit.
+#include <algorithm>
 #include "fp4.h"
 
 namespace {
@@ -52,9 +53,9 @@ __global__ __launch_bounds__(256) void clear_columns_kernel(uint16_t* __restrict
   if (at < rows * (ld - I)) h[at / (ld - I) * ld + I + at % (ld - I)] = 0;
 }
 
-// Up to 16 rows run through the kernel that has no barriers (fp4_few.hip), but from 9 on not where the weight is large: 16 rows of 37888 x 3584
-// 25.5 us there, 22.1 in tiles of 32 rows; 3584 x 18944 23.5 and 19.4; 4608 x 3584 7.6 and 10.2.
-bool few_rows(int M, int N, int K) { return M <= 8 || (M <= 16 && (int64_t)N * K < (60 << 20)); }
+// Up to 16 rows run through the kernel that has no barriers (fp4_few.hip): 16 rows of 37888 x 3584 20.2 us, 22.1 in tiles of 32 rows; 3584 x 18944
+// 16.4 and 19.4; 4608 x 3584 6.4 and 10.2.
+constexpr int FEW_ROWS = 16;
 
 // How a product of more rows is cut: a tile's time is its blocks of 128 k times the microseconds that a block takes, alone on its unit or as its
 // share of a unit that has several; the fewest over the shapes and the slices of K, whose sums cost two passes over them and a
@@ -83,7 +84,7 @@ struct ProductScratch {
 };
 ProductScratch product_scratch(int M, int N, int K) {
   ProductScratch t = {{0, 0, 1}, 0, 0};
-  if (few_rows(M, N, K)) return t;
+  if (M <= FEW_ROWS) return t;
   t.plan = plan_of(M, N, K);
   t.rows = K % FP4_K ? padded(M * padded_k(K) * 2) : 0;
   t.bytes = t.rows + (t.plan.slices > 1 ? (int64_t)t.plan.slices * M * ((N + 15) / 16 * 16) * 4 : 0);
@@ -165,7 +166,7 @@ extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx
   c.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic};
   c.pairs = ldo % (gated ? 2 : 4) == 0 && ((uintptr_t)out & (out_dtype == HE_F32 ? 15 : gated ? 3 : 7)) == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (few_rows(M, N, K)) return fp4_run_few(c, 1, s);
+  if (M <= FEW_ROWS) return fp4_run_few(c, 1, s);
   const ProductScratch t = product_scratch(M, N, K);
   HE_REQUIRE(t.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= t.bytes),
              "he_fp4_product: a workspace of %lld bytes, 16-byte aligned, is needed", (long long)t.bytes);
@@ -216,6 +217,7 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
   down.out = partial, down.ldo = D, down.out_f32 = true, down.pairs = D % 4 == 0;
   down.tile_begin = lists.tile_begin, down.groups = experts, down.rows_of = down.out_of = lists.choice_of;
   if (t.bm == 16) {
+    up.M = down.M = (int)std::min<int64_t>((int64_t)rows * top, 1 << 20);
     if ((rc = fp4_run_few(up, t.mtiles, s)) || (rc = fp4_run_few(down, t.mtiles, s))) return rc;
   } else {
     if (D % FP4_K || !up.whole || far(rows, ldx)) {
