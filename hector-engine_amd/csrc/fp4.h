@@ -54,13 +54,16 @@ struct Fp4Case {
   bool out_f32, gated;
   const void* bias;           // [N] or null
   int bias_dtype;
-  int M;                      // with groups: the most slots that a group can have
+  int M;
   GatedAct act;
+  const int32_t* ids;         // [choices]: an expert each (fewer than groups, or none); a choice's row is choice / top, its results row `choice`. Or null
+  const float* shares;        // [choices]: one of zero is left out
+  int choices, top;
   const int32_t* tile_begin;  // [groups + 1]: a group's first tile of slots; null: no groups
   int groups;
   const int32_t* rows_of;     // a slot's row of x, -1: none
   const int32_t* out_of;      // a slot's row of out, -1: none
-  const float* factor;        // what a slot's results are multiplied by, or null
+  const float* factor;        // what a slot's (with ids: a choice's) results are multiplied by, or null
   bool pairs;                 // out takes stores of four neighbouring results (gated: of two)
 };
 
@@ -126,8 +129,10 @@ __device__ __forceinline__ int fp4_group_of(const int32_t* tile_begin, int group
   return lo;
 }
 
-// fp4_few.hip: rows in tiles of 16, of which the first M are real
-int fp4_run_few(const Fp4Case& c, int mtiles, hipStream_t s);
+// fp4_few.hip: rows in tiles of bm (4, 8 or 16)
+int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s);
+// one row, the sum over its choices (with ids): of expert ids[choice] with X row `choice`
+int fp4_run_chain(const Fp4Case& c, hipStream_t s);
 // fp4_tall.hip: rows in tiles of 16 mt, mtiles of them at most, weight rows in tiles of 64 nt; x may be read 16 bytes at a time, K is a multiple of
 // 128. slices > 1: K cut in so many (of a block at least), their sums by way of parts [slices][M][N rounded up to 16].
 struct Fp4Plan {

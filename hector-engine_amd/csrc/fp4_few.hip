@@ -8,60 +8,89 @@ namespace {
 // wavefront's own part of LDS into the order of the operands: read as operands from memory, each of its rows a sixteen-byte piece a
 // lane and all 16 of them whatever X has, it took a third of the time (8 rows of 37888 x 3584 19.5 us, without it 14).
 // There the pieces of a row lie at their index xor the row, so that the rows of an operand are in different banks.
-template <int NT, int W, int D, int XL, int GROUPS, bool WHOLE>
+// With ids (64 choices at most) a tile's slots are found here, by every wavefront for itself: slot by slot the choices of one expert, the
+// tiles in the order of their first choices. CHAIN: one row and all of its choices, a tile's sums taken over the choices' K one after the
+// other (codes of expert ids[choice], X row `choice`), so that nothing is left to add up.
+template <int NT, int W, int D, int XL, int GROUPS, bool WHOLE, bool CHAIN>
 __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[W * (NT > 2 * XL ? NT : 2 * XL) * 1024];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
-  const int blocks = c.w.blocks, lo = blocks * wave / W, hi = blocks * (wave + 1) / W;
+  constexpr int ROWS = 4 * XL;                             // of a tile of rows
+  __shared__ int32_t choice_in[W][16];                     // with ids: a slot's choice, -1: none
+  const int blocks = c.w.blocks, units = CHAIN ? c.choices * blocks : blocks;      // (a unit: a block of a choice)
+  const int lo = units * wave / W, hi = units * (wave + 1) / W;
   int group = 0;
+  int id = -1;                                             // lane i: the expert of choice i, -1: none
+  if (c.ids) {
+    if (lane < c.choices && c.shares[lane] != 0.f) id = c.ids[lane];
+    if (id >= c.groups) id = -1;
+  }
   if (c.tile_begin) {
     if ((int)blockIdx.y >= c.tile_begin[c.groups]) return;
     group = fp4_group_of(c.tile_begin, c.groups, blockIdx.y);
+  } else if (c.ids && !CHAIN) {
+    int rank = 0;                                          // choices of the same expert in front
+    for (int j = 0; j < c.choices - 1; ++j) rank += j < lane && __builtin_amdgcn_readlane(id, j) == id;
+    uint64_t first = __ballot(id >= 0 && rank % ROWS == 0);
+    if (__popcll(first) <= (int)blockIdx.y) return;        // (the same in all wavefronts)
+    for (int i = 0; i < (int)blockIdx.y; ++i) first &= first - 1;
+    const int lead = __ffsll((unsigned long long)first) - 1;
+    group = __builtin_amdgcn_readlane(id, lead);
+    const int base = __builtin_amdgcn_readlane(rank, lead);
+    if (lane < 16) choice_in[wave][lane] = -1;
+    if (id == group && rank >= base && rank < base + ROWS) choice_in[wave][rank - base] = lane;
   }
-  const int m0 = blockIdx.y * 16, tile0 = blockIdx.x * NT;
-  const uint8_t* codes[NT];
-  const uint16_t* scales[NT];
+  const int m0 = blockIdx.y * ROWS, tile0 = blockIdx.x * NT;
+  int64_t tile_at[NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int64_t at = ((int64_t)group * c.w.tiles + min(tile0 + j, c.w.tiles - 1)) * blocks;
-    codes[j] = c.w.codes + at * FP4_TILE_BYTES;
-    scales[j] = c.w.scales + at * (16 * GROUPS);
-  }
+  for (int j = 0; j < NT; ++j) tile_at[j] = ((int64_t)group * c.w.tiles + min(tile0 + j, c.w.tiles - 1)) * blocks;
   // a lane's pieces of X: row 4 i + (lane >> 4), eight k from 8 (lane & 15) on (rows behind the last repeat it: each row's results are its own)
   const uint16_t* x[XL];
 #pragma unroll
   for (int i = 0; i < XL; ++i) {
     const int slot = m0 + 4 * i + kq;
-    x[i] = c.x + (c.rows_of ? (int64_t)max(c.rows_of[slot], 0) : min(slot, c.M - 1)) * c.ldx;
+    x[i] = c.x;
+    if (c.ids && !CHAIN) x[i] += (int64_t)(max(choice_in[wave][4 * i + kq], 0) / c.top) * c.ldx;
+    else if (!CHAIN) x[i] += (c.rows_of ? (int64_t)max(c.rows_of[slot], 0) : min(slot, c.M - 1)) * c.ldx;
   }
   const int K = c.w.K;
   uint8_t* own = lds + wave * (2 * XL * 1024);
 
   uint4 q[D][NT], xs[D][XL];
   uint2 s[D][NT][GROUPS];
-  auto load = [&](int u, int kb) {
+  auto load = [&](int u, int unit) {
+    int kb = unit;
+    int64_t from = 0, xfrom = 0;
+    if (CHAIN) {
+      const int choice = unit / blocks;
+      kb = unit - choice * blocks;
+      from = (int64_t)max(__builtin_amdgcn_readlane(id, choice), 0) * c.w.tiles * blocks;
+      xfrom = choice * c.ldx;
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      q[u][j] = he_load16_once<uint4>(codes[j] + (int64_t)kb * FP4_TILE_BYTES + lane * 16);
+      const int64_t at = tile_at[j] + from + kb;
+      q[u][j] = he_load16_once<uint4>(c.w.codes + at * FP4_TILE_BYTES + lane * 16);
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) s[u][j][g] = *reinterpret_cast<const uint2*>(scales[j] + (int64_t)kb * (16 * GROUPS) + 16 * g + 4 * kq);
+      for (int g = 0; g < GROUPS; ++g) s[u][j][g] = *reinterpret_cast<const uint2*>(c.w.scales + at * (16 * GROUPS) + 16 * g + 4 * kq);
     }
     const int k = kb * FP4_K + 8 * r16;
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
       if (WHOLE) {
-        xs[u][i] = *reinterpret_cast<const uint4*>(x[i] + min(k, K - 8));
+        xs[u][i] = *reinterpret_cast<const uint4*>(x[i] + xfrom + min(k, K - 8));
       } else {
         uint32_t words[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (k + e < K) words[e >> 1] |= (uint32_t)x[i][k + e] << (16 * (e & 1));
+          if (k + e < K) words[e >> 1] |= (uint32_t)x[i][xfrom + k + e] << (16 * (e & 1));
         xs[u][i] = make_uint4(words[0], words[1], words[2], words[3]);
       }
     }
   };
   // X of a block into one of two places
-  auto keep = [&](int u, int kb, int place) {
+  auto keep = [&](int u, int unit, int place) {
+    const int kb = CHAIN ? unit % blocks : unit;
     const bool behind = WHOLE && kb * FP4_K + 8 * r16 >= K;
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
@@ -73,7 +102,8 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   fp4_f32x4 acc[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j] = fp4_f32x4{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](int u, int place) {
+  auto multiply = [&](int u, int unit, int place) {
+    if (CHAIN && __builtin_amdgcn_readlane(id, unit / blocks) < 0) return;      // (a choice of no expert adds nothing)
     fp4_bf16x8 v[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -104,7 +134,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
 #pragma unroll
       for (int u = 0; u < D; ++u) {
         keep(u, kb + u, u & 1);
-        multiply(u, u & 1);
+        multiply(u, kb + u, u & 1);
         load(u, min(kb + D + u, hi - 1));
       }
     }
@@ -112,7 +142,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     for (int u = 0; u < D; ++u)
       if (kb + u < hi) {
         keep(u, kb + u, u & 1);
-        multiply(u, u & 1);
+        multiply(u, kb + u, u & 1);
       }
   }
   __syncthreads();
@@ -121,7 +151,10 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   __syncthreads();
   const int slot = m0 + r16;
   int to = slot;
-  if (c.out_of) to = c.out_of[slot];
+  if (r16 >= ROWS) to = -1;
+  else if (CHAIN) to = r16 == 0 ? 0 : -1;
+  else if (c.ids) to = choice_in[wave][r16];
+  else if (c.out_of) to = c.out_of[slot];
   else if (slot >= c.M) to = -1;
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -130,16 +163,16 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
 #pragma unroll
     for (int k = 0; k < W; ++k) v += *reinterpret_cast<const fp4_f32x4*>(lds + (k * NT + j) * 1024 + lane * 16);
     const int n = (tile0 + j) * FP4_ROWS + 4 * kq;
-    if (to >= 0 && n < c.w.N) fp4_store(c, v, to, n, c.factor ? c.factor[slot] : 1.f);
+    if (to >= 0 && n < c.w.N) fp4_store(c, v, to, n, c.factor ? c.factor[c.ids ? to : slot] : 1.f);
   }
 }
 
-template <int NT, int W, int D, int XL, bool WHOLE>
+template <int NT, int W, int D, int XL, bool WHOLE, bool CHAIN = false>
 int run_few(const Fp4Case& c, int mtiles, hipStream_t s) {
   const dim3 grid((c.w.tiles + NT - 1) / NT, mtiles);
-  if (c.w.group == 128) fp4_few_kernel<NT, W, D, XL, 1, WHOLE><<<grid, 64 * W, 0, s>>>(c);
-  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, XL, 2, WHOLE><<<grid, 64 * W, 0, s>>>(c);
-  else fp4_few_kernel<NT, W, D, XL, 4, WHOLE><<<grid, 64 * W, 0, s>>>(c);
+  if (c.w.group == 128) fp4_few_kernel<NT, W, D, XL, 1, WHOLE, CHAIN><<<grid, 64 * W, 0, s>>>(c);
+  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, XL, 2, WHOLE, CHAIN><<<grid, 64 * W, 0, s>>>(c);
+  else fp4_few_kernel<NT, W, D, XL, 4, WHOLE, CHAIN><<<grid, 64 * W, 0, s>>>(c);
   return he_check_launch("he_fp4_product");
 }
 
@@ -162,7 +195,14 @@ int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
 
 }  // namespace
 
-int fp4_run_few(const Fp4Case& c, int mtiles, hipStream_t s) {
+int fp4_run_chain(const Fp4Case& c, hipStream_t s) {
+  HE_REQUIRE(c.ids && c.choices >= 1 && c.choices <= 64 && c.M == 1, "he_fp4_experts: %d choices of a row", c.choices);
+  if (!c.whole || c.w.K % 8) return run_few<1, 8, 2, 1, false, true>(c, 1, s);
+  return c.w.tiles <= 256 ? run_few<1, 8, 2, 1, true, true>(c, 1, s) : run_few<2, 8, 2, 1, true, true>(c, 1, s);
+}
+
+int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s) {
+  HE_REQUIRE(!c.ids || c.choices <= 64, "he_fp4_experts: %d choices to be grouped by each workgroup", c.choices);
   HE_REQUIRE(mtiles <= 65535, "he_fp4_product: %d tiles of rows are too many for one launch", mtiles);
-  return c.M > 8 ? run_rows<4>(c, mtiles, s) : c.M > 4 ? run_rows<2>(c, mtiles, s) : run_rows<1>(c, mtiles, s);
+  return bm > 8 ? run_rows<4>(c, mtiles, s) : bm > 4 ? run_rows<2>(c, mtiles, s) : run_rows<1>(c, mtiles, s);
 }

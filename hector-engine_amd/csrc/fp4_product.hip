@@ -101,14 +101,14 @@ struct ExpertsScratch {
 ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   ExpertsScratch t = {};
   const int64_t choices = (int64_t)rows * top;
-  // A tile of rows should hold an expert's rows, of which there are more with some experts than with others. Microseconds in tiles of 16, 32, 64,
-  // 128 rows of 16 experts of 2048 over rows of 2048, 4 chosen: 32 rows 41, 42, 51, 100; 64 rows 54, 44, 51, 100; 256 rows 125, 76, 74, 113;
-  // 512 rows 219, 128, 119, 128; 2048 rows 800, 464, 418, 303.
-  t.bm = choices <= 8ll * experts ? 16 : choices <= 40ll * experts ? 32 : choices <= 96ll * experts ? 64 : 128;
+  // A tile of rows should hold an expert's rows, of which there are more with some experts than with others. Microseconds in tiles of 4, 16, 32, 64,
+  // 128 rows of 16 experts of 2048 over rows of 2048, 4 chosen: 4 rows 30, 35, 39; 8 rows 38, 43, 46; 16 rows 42, 42, 46; 32 rows 60, 44, 43, 51, 100;
+  // 64 rows 89, 54, 46, 51, 100; 256 rows -, 125, 76, 74, 113; 512 rows -, 219, 128, 119, 128; 2048 rows -, 800, 464, 418, 303.
+  t.bm = choices <= 3ll * experts ? 4 : choices <= 8ll * experts ? 16 : choices <= 40ll * experts ? 32 : choices <= 96ll * experts ? 64 : 128;
   t.mtiles = he_group_rows_most_tiles(rows, top, experts, t.bm);
   t.up = t.down = {t.bm / 16, t.bm == 128 ? 4 : 1, 1};
   t.ints = padded(4 * he_group_rows_ints(rows, top, experts, t.bm));
-  t.ldh = t.bm == 16 ? I : padded_k(I);
+  t.ldh = t.bm <= 16 ? I : padded_k(I);
   t.h = padded(choices * t.ldh * 2);
   t.partial = padded(choices * D * 4);
   t.x = t.bm > 16 ? padded(rows * padded_k(D) * 2) : 0;
@@ -116,7 +116,7 @@ ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   return t;
 }
 
-// out[row] = the sum over the row's choices, in their order, of those that an expert took, and of weight * x of those from `experts` on (x null:
+// out[row] = the sum over the row's choices, in their order, of those that an expert took (with a weight that is not zero), and of weight * x of those from `experts` on (x null:
 // they add nothing)
 __global__ __launch_bounds__(256) void add_choices_kernel(uint16_t* __restrict__ out, const float* __restrict__ partial, const int32_t* __restrict__ ids,
                                                           const float* __restrict__ weights, const uint16_t* __restrict__ x, int64_t ldx, int top,
@@ -131,8 +131,8 @@ __global__ __launch_bounds__(256) void add_choices_kernel(uint16_t* __restrict__
     const int id = ids[choice];
     if (id < 0 || (id >= experts && !x)) continue;
     const float w = weights[choice];
+    if (w == 0.f) continue;
     if (id >= experts) {
-      if (w == 0.f) continue;
       for (int i = 0; i < n; ++i) sum[i] = fmaf(w, bf16_bits_to_float(x[row * ldx + d + i]), sum[i]);
     } else if (D % 4 == 0) {
       const float4 v = *reinterpret_cast<const float4*>(partial + choice * D + d);
@@ -166,13 +166,13 @@ extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx
   c.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic};
   c.pairs = ldo % (gated ? 2 : 4) == 0 && ((uintptr_t)out & (out_dtype == HE_F32 ? 15 : gated ? 3 : 7)) == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (M <= FEW_ROWS) return fp4_run_few(c, 1, s);
+  if (M <= FEW_ROWS) return fp4_run_few(c, M > 8 ? 16 : M > 4 ? 8 : 4, 1, s);
   const ProductScratch t = product_scratch(M, N, K);
   HE_REQUIRE(t.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= t.bytes),
              "he_fp4_product: a workspace of %lld bytes, 16-byte aligned, is needed", (long long)t.bytes);
   if (K % FP4_K == 0 && (!c.whole || far(M, ldx))) {
     // rows that cannot be read 16 bytes at a time or lie gigabytes apart, and have no room in the workspace: 16 at a time
-    return fp4_run_few(c, (M + 15) / 16, s);
+    return fp4_run_few(c, 16, (M + 15) / 16, s);
   }
   if (K % FP4_K) {
     HE_REQUIRE(!far(M, padded_k(K)), "he_fp4_product: %d rows of %d are too many", M, K);
@@ -204,9 +204,13 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
              (long long)t.bytes);
   hipStream_t s = (hipStream_t)stream;
   uint8_t* p = (uint8_t*)workspace;
-  GroupRows lists;
-  int rc = he_group_rows(&lists, p, ids_i32, weights_f32, rows, top, experts, t.bm, stream);
-  if (rc) return rc;
+  const int choices = rows * top;
+  // few choices are grouped by the products themselves: a launch less (1 row of 16 experts of 2048 over rows of 2048, 4 chosen, 18.9 us -> 15.0,
+  // its second product's sums taken over the choices too); by more than 16 every workgroup would search for longer than the launch takes
+  const bool by_ids = t.bm <= 16 && choices <= 16;
+  GroupRows lists = {};
+  int rc = 0;
+  if (!by_ids && (rc = he_group_rows(&lists, p, ids_i32, weights_f32, rows, top, experts, t.bm, stream))) return rc;
   uint16_t* h = (uint16_t*)(p + t.ints);
   float* partial = (float*)(p + t.ints + t.h);
   up.x = (const uint16_t*)x, up.ldx = ldx, up.whole = whole_rows(x, ldx), up.M = rows;
@@ -216,9 +220,18 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
   down.x = h, down.ldx = t.ldh, down.whole = whole_rows(h, t.ldh);
   down.out = partial, down.ldo = D, down.out_f32 = true, down.pairs = D % 4 == 0;
   down.tile_begin = lists.tile_begin, down.groups = experts, down.rows_of = down.out_of = lists.choice_of;
-  if (t.bm == 16) {
-    up.M = down.M = (int)std::min<int64_t>((int64_t)rows * top, 1 << 20);
-    if ((rc = fp4_run_few(up, t.mtiles, s)) || (rc = fp4_run_few(down, t.mtiles, s))) return rc;
+  if (t.bm <= 16) {
+    if (by_ids) {
+      up.ids = down.ids = (const int32_t*)ids_i32, up.choices = down.choices = choices, up.top = top, down.top = 1;
+      up.shares = down.shares = up.factor = (const float*)weights_f32;
+      if (rows == 1 && !identity) {
+        down.M = 1, down.out = out, down.out_f32 = false;
+        down.pairs = D % 4 == 0 && ((uintptr_t)out & 7) == 0;
+        if ((rc = fp4_run_few(up, t.bm, t.mtiles, s))) return rc;
+        return fp4_run_chain(down, s);
+      }
+    }
+    if ((rc = fp4_run_few(up, t.bm, t.mtiles, s)) || (rc = fp4_run_few(down, t.bm, t.mtiles, s))) return rc;
   } else {
     if (D % FP4_K || !up.whole || far(rows, ldx)) {
       if ((rc = pad_rows(&up, p + t.ints + t.h + t.partial, s))) return rc;

@@ -181,6 +181,8 @@ def experts_case(seed, rows, E, top, I, D, group, act, holes=True):
 @pytest.mark.parametrize("rows,E,top,I,D,group,act", [
     (1, 2, 1, 8, 16, 32, (1.0, 0.0, 0.0)), (1, 16, 4, 40, 64, 64, (1.0, 0.0, 0.0)), (5, 8, 3, 24, 72, 32, (1.702, 7.0, 1.0)),
     (20, 3, 3, 136, 128, 128, (1.0, 0.0, 0.0)), (64, 4, 2, 64, 200, 32, (1.0, 0.0, 0.0)), (130, 2, 2, 48, 40, 64, (1.0, 0.0, 0.0)),
+    (1, 5, 8, 136, 72, 32, (1.702, 7.0, 1.0)), (1, 4, 3, 20, 36, 64, (1.0, 0.0, 0.0)), (1, 3, 64, 24, 40, 32, (1.0, 0.0, 0.0)),
+    (20, 16, 4, 72, 136, 32, (1.0, 0.0, 0.0)), (16, 2, 4, 40, 80, 64, (1.0, 0.0, 0.0)), (40, 64, 2, 16, 48, 32, (1.0, 0.0, 0.0)),
     (150, 7, 2, 20, 36, 32, (1.702, 7.0, 1.0)), (3, 200, 8, 8, 16, 32, (1.0, 0.0, 0.0)), (400, 3, 2, 144, 264, 128, (1.0, 0.0, 0.0))])
 def test_experts(api, rows, E, top, I, D, group, act):
     fp4, ops = api
@@ -219,6 +221,31 @@ def test_experts_the_same_expert_twice_and_a_row_without_numbers(api):
     got = run(bad, ids, shares)
     keep = torch.tensor([0, 1, 2, 4, 5])
     assert torch.equal(got[keep], clean[keep]) and got[3].isnan().all()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40, 200])
+def test_experts_identity_ids_that_are_none_and_weights_of_zero(api, rows):
+    """An id from E on takes weight * x with identity and nothing without; below 0 nothing; a weight of 0 nothing, whatever the expert holds."""
+    fp4, ops = api
+    E, I, D, top = 5, 40, 72, 3
+    gu, dn, x = rnd(90, E, 2 * I, D, scale=0.1), rnd(91, E, D, I, scale=0.1), rnd(92, rows, D)
+    dn[4] = float("nan")                             # (the last expert is chosen with weight 0 alone)
+    up, down = fp4.pack(gu.cuda(), 32), fp4.pack(dn.cuda(), 32)
+    gen = torch.Generator().manual_seed(93)
+    ids = torch.randint(0, 4, (rows, top), generator=gen, dtype=torch.int32)
+    shares = torch.rand((rows, top), generator=gen) + 0.1
+    ids[:, 1], ids[rows // 2, 0] = E + 2, -3
+    ids[rows // 2, 2], shares[rows // 2, 2] = 4, 0.0
+    got = {}
+    for identity in (False, True):
+        out = torch.empty((rows, D), dtype=BF16, device="cuda")
+        ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, identity=identity,
+                        workspace=workspace(ops.fp4_experts_workspace_bytes(rows, top, up, down)))
+        got[identity] = out.cpu().double()
+    assert got[False].isfinite().all() and (got[False][rows // 2] == 0).all()
+    own = shares[:, 1:2].double() * x.double()
+    # each result half a step off, and the sums of 32 bits
+    assert ((got[True] - got[False] - own).abs() <= HALF[BF16] * (got[True].abs() + got[False].abs()) * 1.01 + 2.0 ** -20 * own.abs()).all()
 
 
 def test_a_row_does_not_depend_on_the_rows_beside_it(api):
