@@ -1,4 +1,4 @@
-// Products of up to 16 rows with a weight in 4 bits (fp4.h).
+// Products of few rows with a weight in 4 bits (fp4.h).
 #include "fp4.h"
 
 namespace {
@@ -11,7 +11,7 @@ namespace {
 // With ids (64 choices at most) a tile's slots are found here, by every wavefront for itself: slot by slot the choices of one expert, the
 // tiles in the order of their first choices. CHAIN: one row and all of its choices, a tile's sums taken over the choices' K one after the
 // other (codes of expert ids[choice], X row `choice`), so that nothing is left to add up.
-template <int NT, int W, int D, int XL, int GROUPS, bool WHOLE, bool CHAIN>
+template <int NT, int W, int D, int XL, int GROUPS, bool CHAIN>
 __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[W * (NT > 2 * XL ? NT : 2 * XL) * 1024];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
@@ -76,22 +76,12 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     }
     const int k = kb * FP4_K + 8 * r16;
 #pragma unroll
-    for (int i = 0; i < XL; ++i) {
-      if (WHOLE) {
-        xs[u][i] = *reinterpret_cast<const uint4*>(x[i] + xfrom + min(k, K - 8));
-      } else {
-        uint32_t words[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + e < K) words[e >> 1] |= (uint32_t)x[i][xfrom + k + e] << (16 * (e & 1));
-        xs[u][i] = make_uint4(words[0], words[1], words[2], words[3]);
-      }
-    }
+    for (int i = 0; i < XL; ++i) xs[u][i] = *reinterpret_cast<const uint4*>(x[i] + xfrom + min(k, K - 8));
   };
   // X of a block into one of two places
   auto keep = [&](int u, int unit, int place) {
     const int kb = CHAIN ? unit % blocks : unit;
-    const bool behind = WHOLE && kb * FP4_K + 8 * r16 >= K;
+    const bool behind = kb * FP4_K + 8 * r16 >= K;
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
       const int row = 4 * i + kq;
@@ -167,41 +157,40 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   }
 }
 
-template <int NT, int W, int D, int XL, bool WHOLE, bool CHAIN = false>
+template <int NT, int W, int D, int XL, bool CHAIN = false>
 int run_few(const Fp4Case& c, int mtiles, hipStream_t s) {
   const dim3 grid((c.w.tiles + NT - 1) / NT, mtiles);
-  if (c.w.group == 128) fp4_few_kernel<NT, W, D, XL, 1, WHOLE, CHAIN><<<grid, 64 * W, 0, s>>>(c);
-  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, XL, 2, WHOLE, CHAIN><<<grid, 64 * W, 0, s>>>(c);
-  else fp4_few_kernel<NT, W, D, XL, 4, WHOLE, CHAIN><<<grid, 64 * W, 0, s>>>(c);
+  if (c.w.group == 128) fp4_few_kernel<NT, W, D, XL, 1, CHAIN><<<grid, 64 * W, 0, s>>>(c);
+  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, XL, 2, CHAIN><<<grid, 64 * W, 0, s>>>(c);
+  else fp4_few_kernel<NT, W, D, XL, 4, CHAIN><<<grid, 64 * W, 0, s>>>(c);
   return he_check_launch("he_fp4_product");
 }
 
 template <int XL>
 int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
-  if (!c.whole || c.w.K % 8) return run_few<1, 8, 2, XL, false>(c, mtiles, s);
   // Microseconds of (tiles, wavefronts, blocks ahead) = (1, 8, 2), (1, 8, 4), (2, 4, 2), (2, 8, 2), (4, 4, 2), weights from memory:
   // 1 row of 4608 x 3584 5.0, 5.4, 5.5, 4.8, 7.0; 3584 x 18944 10.5, 9.3, 17.4, 12.4, 23.8; 5120 x 27648 19.8, 20.2, 25.0, 17.6, 33.5; 8 rows of
   // 37888 x 3584 21.2, 23.3, 17.3, 17.6, 18.4; 16 rows of 10240 x 5120 15.3, 20.0, 12.9, 14.0, 10.7, of 3584 x 18944 16.4, 17.1, 20.5, 20.0, 26.5.
   const int64_t tiles = (int64_t)c.w.tiles * mtiles;
   if (tiles <= 256) {
     if constexpr (XL == 1) {
-      if (c.w.blocks >= 64) return run_few<1, 8, 4, XL, true>(c, mtiles, s);
+      if (c.w.blocks >= 64) return run_few<1, 8, 4, XL>(c, mtiles, s);
     }
-    return run_few<1, 8, 2, XL, true>(c, mtiles, s);
+    return run_few<1, 8, 2, XL>(c, mtiles, s);
   }
-  if (XL == 4 && tiles >= 640) return run_few<4, 4, 2, XL, true>(c, mtiles, s);
-  return tiles <= 512 && c.w.blocks >= 64 ? run_few<2, 8, 2, XL, true>(c, mtiles, s) : run_few<2, 4, 2, XL, true>(c, mtiles, s);
+  if (XL == 4 && tiles >= 640) return run_few<4, 4, 2, XL>(c, mtiles, s);
+  return tiles <= 512 && c.w.blocks >= 64 ? run_few<2, 8, 2, XL>(c, mtiles, s) : run_few<2, 4, 2, XL>(c, mtiles, s);
 }
 
 }  // namespace
 
 int fp4_run_chain(const Fp4Case& c, hipStream_t s) {
-  HE_REQUIRE(c.ids && c.choices >= 1 && c.choices <= 64 && c.M == 1, "he_fp4_experts: %d choices of a row", c.choices);
-  if (!c.whole || c.w.K % 8) return run_few<1, 8, 2, 1, false, true>(c, 1, s);
-  return c.w.tiles <= 256 ? run_few<1, 8, 2, 1, true, true>(c, 1, s) : run_few<2, 8, 2, 1, true, true>(c, 1, s);
+  HE_REQUIRE(c.whole && c.w.K % 8 == 0 && c.ids && c.choices >= 1 && c.choices <= 64 && c.M == 1, "he_fp4_experts: %d choices of a row", c.choices);
+  return c.w.tiles <= 256 ? run_few<1, 8, 2, 1, true>(c, 1, s) : run_few<2, 8, 2, 1, true>(c, 1, s);
 }
 
 int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s) {
+  HE_REQUIRE(c.whole && c.w.K % 8 == 0, "he_fp4_product: rows that cannot be read 16 bytes at a time");
   HE_REQUIRE(!c.ids || c.choices <= 64, "he_fp4_experts: %d choices to be grouped by each workgroup", c.choices);
   HE_REQUIRE(mtiles <= 65535, "he_fp4_product: %d tiles of rows are too many for one launch", mtiles);
   return bm > 8 ? run_rows<4>(c, mtiles, s) : bm > 4 ? run_rows<2>(c, mtiles, s) : run_rows<1>(c, mtiles, s);

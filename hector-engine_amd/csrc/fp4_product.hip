@@ -17,7 +17,6 @@ Fp4Weight weight(const void* codes, const void* scales, int N, int K, int group)
 
 bool whole_rows(const void* x, int64_t ldx) { return ((uintptr_t)x & 15) == 0 && ldx % 8 == 0; }
 
-// (the kernels of many rows count in 32 bits from the first row on)
 bool far(int64_t rows, int64_t ld) { return rows * ld * 2 >= 1ll << 32; }
 
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -41,7 +40,8 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(uint4* __restrict__ out, 
     if (8 * p + e < K) words[e >> 1] |= (uint32_t)row[8 * p + e] << (16 * (e & 1));
   out[at] = make_uint4(words[0], words[1], words[2], words[3]);
 }
-// X copied to `to`, its rows filled up to whole blocks
+// X copied to `to`, its rows filled up to whole blocks (rows that cannot be read 16 bytes at a time too: element by element the products took
+// 12.2 us for a row of 4608 x 3584 and 33 for 16, with this 8.1 and 9.2)
 int pad_rows(Fp4Case* c, void* to, hipStream_t s) {
   const int64_t ld = padded_k(c->w.K), total = c->M * (ld / 8);
   pad_rows_kernel<<<(unsigned)((total + 255) / 256), 256, 0, s>>>((uint4*)to, c->x, c->ldx, c->w.K, (int)(ld / 8), total, c->whole);
@@ -53,40 +53,42 @@ __global__ __launch_bounds__(256) void clear_columns_kernel(uint16_t* __restrict
   if (at < rows * (ld - I)) h[at / (ld - I) * ld + I + at % (ld - I)] = 0;
 }
 
-// Up to 16 rows run through the kernel that has no barriers (fp4_few.hip): 16 rows of 37888 x 3584 20.2 us, 22.1 in tiles of 32 rows; 3584 x 18944
-// 16.4 and 19.4; 4608 x 3584 6.4 and 10.2.
-constexpr int FEW_ROWS = 16;
-
-// How a product of more rows is cut: a tile's time is its blocks of 128 k times the microseconds that a block takes, alone on its unit or as its
-// share of a unit that has several; the fewest over the shapes and the slices of K, whose sums cost two passes over them and a
-// launch. (Of 50 products, 17 to 1024 rows of 1024 to 37888 columns and K of 3584 to 27648, what this chooses takes 1.04 of the
-// time of the best of 14 shapes and slices in the geometric mean, 1.33 at most.)
-Fp4Plan plan_of(int64_t mrows, int N, int K) {
+// How a product is cut. Up to 16 rows run through the kernel that has no barriers (fp4_few.hip; 16 rows of 37888 x 3584 20.2 us, 22.1 in tiles of 32
+// rows; 3584 x 18944 16.4 and 19.4), and so do more, 16 at a time, where the weight is small (mt 0): it reads the codes again for
+// each 16, at some 4300 blocks of 128 k of 16 rows a microsecond. Tiles of more rows: a tile's time is its blocks of 128 k times the
+// microseconds that a block takes, alone on its unit or as its share of a unit that has several; the fewest over the shapes and the
+// slices of K, whose sums cost two passes over them and a launch. (64 rows of 1024 x 3584 5.1 us in sixteens, 9.8 in tiles; of 4608 x
+// 3584 12.2, 13.7; of 37888 x 3584 27 in tiles. Of 50 products, 17 to 1024 rows of 1024 to 37888 columns and K of 3584 to 27648, the
+// tiles that this chooses take 1.04 of the time of the best of 14 shapes and slices in the geometric mean, 1.33 at most.)
+Fp4Plan plan_of(int64_t M, int N, int K) {
   static const struct { int mt, nt; double alone, shared; } shapes[] = {{2, 1, 0.45, 0.25}, {4, 1, 0.53, 0.4}, {4, 2, 1.0, 0.63}, {8, 2, 1.35, 1.2}, {8, 4, 2.3, 1.75}};
   const int blocks = (K + FP4_K - 1) / FP4_K, cus = he_cus();
-  Fp4Plan best = {8, 4, 1};
-  double least = 1e30;
+  Fp4Plan best = {0, 0, 1};
+  if (M <= 16 || far(M, padded_k(K))) return best;       // (the kernel of many rows counts in 32 bits)
+  double least = 3 + 0.03 * blocks + (double)((M + 15) / 16 * ((N + 15) / 16) * blocks) / 4300 + (K % 8 ? 2.5 : 0);
   for (const auto& t : shapes) {
-    const int64_t tiles = (mrows + 16 * t.mt - 1) / (16 * t.mt) * ((N + 64 * t.nt - 1) / (64 * t.nt));
+    const int64_t tiles = (M + 16 * t.mt - 1) / (16 * t.mt) * ((N + 64 * t.nt - 1) / (64 * t.nt));
     for (int slices = 1; slices <= 16 && slices <= blocks; slices *= 2) {
-      const double load = tiles * slices > 8 * cus ? (double)tiles * slices / cus : (double)((tiles * slices + cus - 1) / cus), turn = load * t.shared > t.alone ? load * t.shared : t.alone;
-      const double us = (blocks + slices - 1) / slices * turn + (slices > 1 ? 4 + 8e-6 * slices * mrows * N / 4 : 0);
+      const double load = tiles * slices > 8 * cus ? (double)tiles * slices / cus : (double)((tiles * slices + cus - 1) / cus);
+      const double turn = load * t.shared > t.alone ? load * t.shared : t.alone;
+      const double us = 3 + (blocks + slices - 1) / slices * turn + (slices > 1 ? 4 + 8e-6 * slices * M * N / 4 : 0) + (K % FP4_K ? 2.5 : 0);
       if (us < least) least = us, best = {t.mt, t.nt, slices};
     }
   }
   return best;
 }
 
-// The scratch of a product: the rows, where K is not whole blocks, then the slices' sums.
+// The scratch of a product: the rows, where they have to be copied, then the slices' sums.
 struct ProductScratch {
   Fp4Plan plan;
+  bool copy;
   int64_t rows, bytes;
 };
-ProductScratch product_scratch(int M, int N, int K) {
-  ProductScratch t = {{0, 0, 1}, 0, 0};
-  if (M <= FEW_ROWS) return t;
+ProductScratch product_scratch(int M, int N, int K, bool whole) {
+  ProductScratch t;
   t.plan = plan_of(M, N, K);
-  t.rows = K % FP4_K ? padded(M * padded_k(K) * 2) : 0;
+  t.copy = !whole || K % (t.plan.mt ? FP4_K : 8) != 0;
+  t.rows = t.copy ? padded(M * padded_k(K) * 2) : 0;
   t.bytes = t.rows + (t.plan.slices > 1 ? (int64_t)t.plan.slices * M * ((N + 15) / 16 * 16) * 4 : 0);
   return t;
 }
@@ -108,10 +110,10 @@ ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   t.mtiles = he_group_rows_most_tiles(rows, top, experts, t.bm);
   t.up = t.down = {t.bm / 16, t.bm == 128 ? 4 : 1, 1};
   t.ints = padded(4 * he_group_rows_ints(rows, top, experts, t.bm));
-  t.ldh = t.bm <= 16 ? I : padded_k(I);
+  t.ldh = t.bm <= 16 ? (I + 7) / 8 * 8 : padded_k(I);
   t.h = padded(choices * t.ldh * 2);
   t.partial = padded(choices * D * 4);
-  t.x = t.bm > 16 ? padded(rows * padded_k(D) * 2) : 0;
+  t.x = padded(rows * padded_k(D) * 2);
   t.bytes = t.ints + t.h + t.partial + t.x;
   return t;
 }
@@ -146,8 +148,8 @@ __global__ __launch_bounds__(256) void add_choices_kernel(uint16_t* __restrict__
 
 }  // namespace
 
-extern "C" int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int gated) {
-  return M <= 0 || N <= 0 || K <= 0 ? 0 : product_scratch(M, N, K).bytes;
+extern "C" int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int whole) {
+  return M <= 0 || N <= 0 || K <= 0 ? 0 : product_scratch(M, N, K, whole).bytes;
 }
 
 extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M, int N,
@@ -166,18 +168,12 @@ extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx
   c.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic};
   c.pairs = ldo % (gated ? 2 : 4) == 0 && ((uintptr_t)out & (out_dtype == HE_F32 ? 15 : gated ? 3 : 7)) == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (M <= FEW_ROWS) return fp4_run_few(c, M > 8 ? 16 : M > 4 ? 8 : 4, 1, s);
-  const ProductScratch t = product_scratch(M, N, K);
+  const ProductScratch t = product_scratch(M, N, K, c.whole && !far(M, ldx));
   HE_REQUIRE(t.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= t.bytes),
              "he_fp4_product: a workspace of %lld bytes, 16-byte aligned, is needed", (long long)t.bytes);
-  if (K % FP4_K == 0 && (!c.whole || far(M, ldx))) {
-    // rows that cannot be read 16 bytes at a time or lie gigabytes apart, and have no room in the workspace: 16 at a time
-    return fp4_run_few(c, 16, (M + 15) / 16, s);
-  }
-  if (K % FP4_K) {
-    HE_REQUIRE(!far(M, padded_k(K)), "he_fp4_product: %d rows of %d are too many", M, K);
+  if (t.copy)
     if (const int rc = pad_rows(&c, workspace, s)) return rc;
-  }
+  if (t.plan.mt == 0) return fp4_run_few(c, M > 8 ? 16 : M > 4 ? 8 : 4, (M + 15) / 16, s);
   return fp4_run_tall(c, t.plan, (M + 16 * t.plan.mt - 1) / (16 * t.plan.mt), (float*)((uint8_t*)workspace + t.rows), s);
 }
 
@@ -217,31 +213,30 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
   up.out = h, up.ldo = t.ldh, up.pairs = t.ldh % 2 == 0, up.gated = true;
   up.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic};
   up.tile_begin = lists.tile_begin, up.groups = experts, up.rows_of = lists.rows_of, up.out_of = lists.choice_of, up.factor = lists.scale;
-  down.x = h, down.ldx = t.ldh, down.whole = whole_rows(h, t.ldh);
+  down.x = h, down.ldx = t.ldh, down.whole = true;
   down.out = partial, down.ldo = D, down.out_f32 = true, down.pairs = D % 4 == 0;
   down.tile_begin = lists.tile_begin, down.groups = experts, down.rows_of = down.out_of = lists.choice_of;
+  if (D % (t.bm <= 16 ? 8 : FP4_K) || !up.whole || far(rows, ldx))
+    if ((rc = pad_rows(&up, p + t.ints + t.h + t.partial, s))) return rc;
+  if (I != t.ldh) {
+    // (the columns behind I are multiplied with codes of zero: they have to be numbers)
+    clear_columns_kernel<<<(unsigned)(((int64_t)choices * (t.ldh - I) + 255) / 256), 256, 0, s>>>(h, choices, I, (int)t.ldh);
+    if ((rc = he_check_launch("he_fp4_experts (rows)"))) return rc;
+    down.w.K = (int)t.ldh;
+  }
+  if (by_ids) {
+    up.ids = down.ids = (const int32_t*)ids_i32, up.choices = down.choices = choices, up.top = top, down.top = 1;
+    up.shares = down.shares = up.factor = (const float*)weights_f32;
+  }
+  if (by_ids && rows == 1 && !identity) {
+    down.M = 1, down.out = out, down.out_f32 = false;
+    down.pairs = D % 4 == 0 && ((uintptr_t)out & 7) == 0;
+    if ((rc = fp4_run_few(up, t.bm, t.mtiles, s))) return rc;
+    return fp4_run_chain(down, s);
+  }
   if (t.bm <= 16) {
-    if (by_ids) {
-      up.ids = down.ids = (const int32_t*)ids_i32, up.choices = down.choices = choices, up.top = top, down.top = 1;
-      up.shares = down.shares = up.factor = (const float*)weights_f32;
-      if (rows == 1 && !identity) {
-        down.M = 1, down.out = out, down.out_f32 = false;
-        down.pairs = D % 4 == 0 && ((uintptr_t)out & 7) == 0;
-        if ((rc = fp4_run_few(up, t.bm, t.mtiles, s))) return rc;
-        return fp4_run_chain(down, s);
-      }
-    }
     if ((rc = fp4_run_few(up, t.bm, t.mtiles, s)) || (rc = fp4_run_few(down, t.bm, t.mtiles, s))) return rc;
   } else {
-    if (D % FP4_K || !up.whole || far(rows, ldx)) {
-      if ((rc = pad_rows(&up, p + t.ints + t.h + t.partial, s))) return rc;
-    }
-    if (I % FP4_K) {
-      // (the columns behind I are multiplied with codes of zero: they have to be numbers)
-      clear_columns_kernel<<<(unsigned)(((int64_t)rows * top * (t.ldh - I) + 255) / 256), 256, 0, s>>>(h, (int64_t)rows * top, I, (int)t.ldh);
-      if ((rc = he_check_launch("he_fp4_experts (rows)"))) return rc;
-      down.w.K = (int)t.ldh;
-    }
     if ((rc = fp4_run_tall(up, t.up, t.mtiles, nullptr, s)) || (rc = fp4_run_tall(down, t.down, t.mtiles, nullptr, s))) return rc;
   }
   add_choices_kernel<<<dim3((D + 1023) / 1024, rows), 256, 0, s>>>((uint16_t*)out, partial, (const int32_t*)ids_i32, (const float*)weights_f32,

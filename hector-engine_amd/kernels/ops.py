@@ -1464,9 +1464,10 @@ def fp4_unpack(out, packed) -> None:
                                          packed.group, dtype_code(out.dtype), _stream()))
 
 
-def fp4_product_workspace_bytes(rows: int, w, gated: bool = False) -> int:
-    """Bytes of scratch memory that fp4_product wants for this weight and so many rows (0: none)."""
-    return int(_lib.load().he_fp4_product_workspace_bytes(rows, *w.shape, int(gated)))
+def fp4_product_workspace_bytes(rows: int, w, gated: bool = False, whole: bool = False) -> int:
+    """Bytes of scratch memory that fp4_product wants for this weight and so many rows, gated or not (0: none). whole: each row of x begins at a
+    multiple of 16 bytes, and they span less than 4 GiB, so that none has to be copied for that."""
+    return int(_lib.load().he_fp4_product_workspace_bytes(rows, *w.shape, whole))
 
 
 @_op("fp4_product")
@@ -1490,7 +1491,8 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.
         _need(bias, "fp4_product: bias", shape=(N,))
         _fp4_on("fp4_product", "bias", bias, device)
     L = _lib.load()
-    ws, size = _fp4_workspace("fp4_product", workspace, L.he_fp4_product_workspace_bytes(rows, N, K, gated), device)
+    whole = ldx % 8 == 0 and x.data_ptr() % 16 == 0 and rows * ldx < 1 << 31
+    ws, size = _fp4_workspace("fp4_product", workspace, L.he_fp4_product_workspace_bytes(rows, N, K, whole), device)
     if rows == 0:
         return
     _lib.check(L.he_fp4_product(out.data_ptr(), ldo, x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), rows, N, K, w.group,

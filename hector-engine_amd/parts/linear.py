@@ -214,7 +214,8 @@ class Linear:
         return out
 
     def _fp4(self, out, x, bias, rows: int, ctx: StepContext, **epilogue) -> None:
-        size = ops.fp4_product_workspace_bytes(rows, self.weight, bool(epilogue))
+        size = ops.fp4_product_workspace_bytes(rows, self.weight, bool(epilogue),
+                                              whole=x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and rows * x.stride(0) < 1 << 31)
         ops.fp4_product(out, x, self.weight, bias, rows, workspace=ctx.scratch.transient((size,), torch.uint8) if size else None, **epilogue)
 
     def _run_library(self, x, rows, ctx, bias, out_dtype, out, sink):

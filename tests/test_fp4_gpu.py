@@ -93,6 +93,35 @@ def test_product(api, M, N, K, group):
         assert ((got[:M] - exact).abs() <= bound * (1 + HALF[dtype]) + (HALF[dtype] + 2.0 ** -24) * (exact.abs() + bound)).all()
 
 
+@pytest.mark.parametrize("M,N,K,group", [(100, 4616, 1160, 64), (520, 4625, 1032, 128), (1100, 2052, 1003, 32), (400, 8200, 392, 32), (70, 9001, 3600, 64),
+                                         (48, 12300, 904, 128), (1030, 130, 4100, 64)])
+def test_product_of_large_weights(api, M, N, K, group):
+    """Sizes that the kernel of many rows takes, whole or in slices of K, at columns and k that end inside tiles: bias, gated, rows that lie apart."""
+    fp4, ops = api
+    wide, w, b = rnd(33, M, K + 16), rnd(34, N, K, scale=0.05), rnd(35, N)
+    x = wide[:, 8:8 + K]
+    packed = fp4.pack(w.cuda(), group)
+    values = packed.unpack(F32).cpu().double()
+    want, size = x.double() @ values.t(), P.sum_bound(x, values, group)
+    room = wide.cuda()
+    for rows, xs in ((room[:, 8:8 + K], "apart"), (x.cuda().contiguous(), "together")):
+        ws = workspace(ops.fp4_product_workspace_bytes(M, packed))
+        for dtype in (F32, BF16):
+            out = torch.full((M + 2, N + 3), 7.0, dtype=dtype, device="cuda")
+            ops.fp4_product(out[1:M + 1, 1:N + 1], rows, packed, b.cuda(), M, workspace=ws)
+            full = want + b.double()
+            off = (out[1:M + 1, 1:N + 1].cpu().double() - full).abs() - (size + HALF[dtype] * full.abs() + 2.0 ** -23 * full.abs())
+            assert off.max() <= 0, (xs, dtype, float(off.max()))
+            out[1:M + 1, 1:N + 1] = 7
+            assert (out == 7).all()                  # nothing beside the results
+        if N % 2 == 0:
+            got = torch.empty((M, N // 2), dtype=BF16, device="cuda")
+            ops.fp4_product(got, rows, packed, None, M, gated=True, workspace=ws)
+            g, u, full = want[:, 0::2].abs(), want[:, 1::2].abs(), P.act(want)
+            slack = 1.13 * size[:, 0::2] * (u + size[:, 1::2]) + (g + size[:, 0::2]) * size[:, 1::2] + 2.0 ** -20 * g * u * (1 + g)      # (as in test_gated_product)
+            assert ((got.cpu().double() - full).abs() <= slack + HALF[BF16] * (full.abs() + slack) + 2.0 ** -120).all(), xs
+
+
 @pytest.mark.parametrize("act", [(1.0, 0.0, 0.0), (1.702, 7.0, 1.0)])
 @pytest.mark.parametrize("M,N,K", [(1, 2, 32), (3, 34, 200), (16, 512, 384), (17, 130, 136), (64, 320, 1024), (130, 258, 264), (260, 1028, 520)])
 def test_gated_product(api, M, N, K, act):
