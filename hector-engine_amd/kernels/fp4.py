@@ -42,6 +42,9 @@ class Fp4Weight:
                 raise ValueError(f"fp4: {what} must be contiguous tensors on one GPU")
             if t.dtype != dtype or tuple(t.shape) != want:
                 raise ValueError(f"fp4: {what} of a matrix {shape} in groups of {group} are {dtype} {want}, not {t.dtype} {tuple(t.shape)}")
+        self._hold(codes, scales, shape, group)
+
+    def _hold(self, codes, scales, shape, group) -> None:
         self._codes, self._scales, self._shape, self._group, self._index = codes, scales, shape, group, codes.get_device()
 
     codes = property(lambda self: self._codes)
@@ -72,10 +75,11 @@ class Fp4Weight:
 def pack(w: torch.Tensor, group: int = 64) -> Fp4Weight:
     """Packs a float32 or bfloat16 matrix on the GPU (the rows of a matrix [N, K] may lie apart)."""
     from . import ops
-    codes, scales = storage_shapes(tuple(w.shape), group)
+    shape, device = tuple(w.shape), w.device
+    codes, scales = storage_shapes(shape, group)
     if not w.is_cuda:
         raise ValueError("fp4.pack: expected a GPU tensor")
-    packed = Fp4Weight(torch.empty(codes, dtype=torch.uint8, device=w.device),
-                       torch.empty(scales, dtype=torch.bfloat16, device=w.device), tuple(w.shape), group)
+    packed = Fp4Weight.__new__(Fp4Weight)      # (its tensors are made here as its checks would have them)
+    packed._hold(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.bfloat16, device=device), shape, group)
     ops.fp4_pack(packed, w)
     return packed

@@ -1401,7 +1401,7 @@ def _fp4_weight(name: str, w, dims: int) -> int:
         raise TypeError(f"{name}: expected a packed weight (kernels.fp4.pack), got {type(w).__name__}")
     if len(w.shape) != dims:
         raise ValueError(f"{name}: expected a packed weight of {dims} dims, got {w.shape}")
-    device = torch.cuda.current_device()
+    device = torch._C._cuda_getDevice()
     if w.device_index != device:
         raise ValueError(f"{name}: a weight on cuda:{w.device_index}, the current device is cuda:{device}")
     return device
