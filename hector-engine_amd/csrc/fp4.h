@@ -129,7 +129,7 @@ __device__ __forceinline__ int fp4_group_of(const int32_t* tile_begin, int group
   return lo;
 }
 
-// fp4_few.hip: rows in tiles of bm (4, 8 or 16); x may be read 16 bytes at a time, K is a multiple of 8
+// fp4_few.hip: rows in tiles of bm (4, 8 or 16); K is 8 at least
 int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s);
 // one row, the sum over its choices (with ids): of expert ids[choice] with X row `choice`
 int fp4_run_chain(const Fp4Case& c, hipStream_t s);

@@ -3,6 +3,11 @@
 
 namespace {
 
+// eight values of X wherever they begin: the unit takes loads of sixteen bytes at any element
+struct __attribute__((packed, aligned(2))) Piece {
+  uint4 v;
+};
+
 // A workgroup has NT tiles of 16 weight rows; its W wavefronts cut K among them, and their sums meet in LDS. Codes, scales and X (4 XL rows of it)
 // come straight into registers, D blocks of 128 k ahead, with no barrier before the end. A block of X goes from there through a
 // wavefront's own part of LDS into the order of the operands: read as operands from memory, each of its rows a sixteen-byte piece a
@@ -76,16 +81,24 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     }
     const int k = kb * FP4_K + 8 * r16;
 #pragma unroll
-    for (int i = 0; i < XL; ++i) xs[u][i] = *reinterpret_cast<const uint4*>(x[i] + xfrom + min(k, K - 8));
+    for (int i = 0; i < XL; ++i) xs[u][i] = reinterpret_cast<const Piece*>(x[i] + xfrom + min(k, K - 8))->v;
   };
   // X of a block into one of two places
   auto keep = [&](int u, int unit, int place) {
     const int kb = CHAIN ? unit % blocks : unit;
-    const bool behind = kb * FP4_K + 8 * r16 >= K;
+    const int over = kb * FP4_K + 8 * r16 + 8 - K;         // (a piece over the end of its row was loaded from the row's last eight values)
+    const bool last = (kb + 1) * FP4_K > K;
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
       const int row = 4 * i + kq;
-      *reinterpret_cast<uint4*>(own + place * (XL * 1024) + row * 256 + (r16 ^ row) * 16) = behind ? make_uint4(0, 0, 0, 0) : xs[u][i];
+      uint4 v = xs[u][i];
+      if (last && over > 0) {
+        const uint64_t a = (uint64_t)v.y << 32 | v.x, b = (uint64_t)v.w << 32 | v.z;
+        const int bits = 16 * over;
+        const uint64_t lo = bits < 64 ? a >> bits | b << (64 - bits) : bits < 128 ? b >> (bits - 64) : 0, hi = bits < 64 ? b >> bits : 0;
+        v = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+      }
+      *reinterpret_cast<uint4*>(own + place * (XL * 1024) + row * 256 + (r16 ^ row) * 16) = v;
     }
   };
   const int xrow = min(r16, 4 * XL - 1);
@@ -185,12 +198,12 @@ int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
 }  // namespace
 
 int fp4_run_chain(const Fp4Case& c, hipStream_t s) {
-  HE_REQUIRE(c.whole && c.w.K % 8 == 0 && c.ids && c.choices >= 1 && c.choices <= 64 && c.M == 1, "he_fp4_experts: %d choices of a row", c.choices);
+  HE_REQUIRE(c.w.K >= 8 && c.ids && c.choices >= 1 && c.choices <= 64 && c.M == 1, "he_fp4_experts: %d choices of a row", c.choices);
   return c.w.tiles <= 256 ? run_few<1, 8, 2, 1, true>(c, 1, s) : run_few<2, 8, 2, 1, true>(c, 1, s);
 }
 
 int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s) {
-  HE_REQUIRE(c.whole && c.w.K % 8 == 0, "he_fp4_product: rows that cannot be read 16 bytes at a time");
+  HE_REQUIRE(c.w.K >= 8, "he_fp4_product: rows of fewer than 8 values");
   HE_REQUIRE(!c.ids || c.choices <= 64, "he_fp4_experts: %d choices to be grouped by each workgroup", c.choices);
   HE_REQUIRE(mtiles <= 65535, "he_fp4_product: %d tiles of rows are too many for one launch", mtiles);
   return bm > 8 ? run_rows<4>(c, mtiles, s) : bm > 4 ? run_rows<2>(c, mtiles, s) : run_rows<1>(c, mtiles, s);

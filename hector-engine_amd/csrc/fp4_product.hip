@@ -40,8 +40,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(uint4* __restrict__ out, 
     if (8 * p + e < K) words[e >> 1] |= (uint32_t)row[8 * p + e] << (16 * (e & 1));
   out[at] = make_uint4(words[0], words[1], words[2], words[3]);
 }
-// X copied to `to`, its rows filled up to whole blocks (rows that cannot be read 16 bytes at a time too: element by element the products took
-// 12.2 us for a row of 4608 x 3584 and 33 for 16, with this 8.1 and 9.2)
+// X copied to `to`, its rows filled up to whole blocks
 int pad_rows(Fp4Case* c, void* to, hipStream_t s) {
   const int64_t ld = padded_k(c->w.K), total = c->M * (ld / 8);
   pad_rows_kernel<<<(unsigned)((total + 255) / 256), 256, 0, s>>>((uint4*)to, c->x, c->ldx, c->w.K, (int)(ld / 8), total, c->whole);
@@ -65,7 +64,7 @@ Fp4Plan plan_of(int64_t M, int N, int K) {
   const int blocks = (K + FP4_K - 1) / FP4_K, cus = he_cus();
   Fp4Plan best = {0, 0, 1};
   if (M <= 16 || far(M, padded_k(K))) return best;       // (the kernel of many rows counts in 32 bits)
-  double least = 3 + 0.03 * blocks + (double)((M + 15) / 16 * ((N + 15) / 16) * blocks) / 4300 + (K % 8 ? 2.5 : 0);
+  double least = 3 + 0.03 * blocks + (double)((M + 15) / 16 * ((N + 15) / 16) * blocks) / 4300;
   for (const auto& t : shapes) {
     const int64_t tiles = (M + 16 * t.mt - 1) / (16 * t.mt) * ((N + 64 * t.nt - 1) / (64 * t.nt));
     for (int slices = 1; slices <= 16 && slices <= blocks; slices *= 2) {
@@ -78,7 +77,7 @@ Fp4Plan plan_of(int64_t M, int N, int K) {
   return best;
 }
 
-// The scratch of a product: the rows, where they have to be copied, then the slices' sums.
+// The scratch of a product: the rows, where the kernel cannot read them as they are, then the slices' sums.
 struct ProductScratch {
   Fp4Plan plan;
   bool copy;
@@ -87,7 +86,7 @@ struct ProductScratch {
 ProductScratch product_scratch(int M, int N, int K, bool whole) {
   ProductScratch t;
   t.plan = plan_of(M, N, K);
-  t.copy = !whole || K % (t.plan.mt ? FP4_K : 8) != 0;
+  t.copy = t.plan.mt ? !whole || K % FP4_K : K < 8;
   t.rows = t.copy ? padded(M * padded_k(K) * 2) : 0;
   t.bytes = t.rows + (t.plan.slices > 1 ? (int64_t)t.plan.slices * M * ((N + 15) / 16 * 16) * 4 : 0);
   return t;
@@ -216,9 +215,9 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
   down.x = h, down.ldx = t.ldh, down.whole = true;
   down.out = partial, down.ldo = D, down.out_f32 = true, down.pairs = D % 4 == 0;
   down.tile_begin = lists.tile_begin, down.groups = experts, down.rows_of = down.out_of = lists.choice_of;
-  if (D % (t.bm <= 16 ? 8 : FP4_K) || !up.whole || far(rows, ldx))
+  if (t.bm <= 16 ? D < 8 : D % FP4_K || !up.whole || far(rows, ldx))
     if ((rc = pad_rows(&up, p + t.ints + t.h + t.partial, s))) return rc;
-  if (I != t.ldh) {
+  if (t.bm <= 16 ? I < 8 : I % FP4_K) {
     // (the columns behind I are multiplied with codes of zero: they have to be numbers)
     clear_columns_kernel<<<(unsigned)(((int64_t)choices * (t.ldh - I) + 255) / 256), 256, 0, s>>>(h, choices, I, (int)t.ldh);
     if ((rc = he_check_launch("he_fp4_experts (rows)"))) return rc;

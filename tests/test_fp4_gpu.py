@@ -122,6 +122,25 @@ def test_product_of_large_weights(api, M, N, K, group):
             assert ((got.cpu().double() - full).abs() <= slack + HALF[BF16] * (full.abs() + slack) + 2.0 ** -120).all(), xs
 
 
+@pytest.mark.parametrize("K", [1, 5, 7, 8, 9, 15, 121, 127, 129, 135, 255, 257])
+@pytest.mark.parametrize("M", [1, 6, 16, 21])
+def test_product_of_rows_that_end_anywhere(api, M, K):
+    """The rows' last values inside a piece of eight, at bases of every alignment; what lies behind and between the rows is NaN."""
+    fp4, ops = api
+    room, w = torch.full((M, 300), float("nan"), dtype=BF16), rnd(37, 40, K, scale=0.1)
+    x = rnd(36, M, K)
+    packed = fp4.pack(w.cuda(), 32)
+    values = P.values(w, 32)
+    want, size = x.double() @ values.T, P.sum_bound(x, values, 32)
+    ws = workspace(ops.fp4_product_workspace_bytes(M, packed))
+    for c0 in (0, 1, 6, 300 - K):
+        room[:] = float("nan")
+        room[:, c0:c0 + K] = x
+        out = torch.empty((M, 40), dtype=F32, device="cuda")
+        ops.fp4_product(out, room.cuda()[:, c0:c0 + K], packed, None, M, workspace=ws)
+        assert ((out.cpu().double() - want).abs() <= size + 2.0 ** -24 * want.abs()).all(), c0
+
+
 @pytest.mark.parametrize("act", [(1.0, 0.0, 0.0), (1.702, 7.0, 1.0)])
 @pytest.mark.parametrize("M,N,K", [(1, 2, 32), (3, 34, 200), (16, 512, 384), (17, 130, 136), (64, 320, 1024), (130, 258, 264), (260, 1028, 520)])
 def test_gated_product(api, M, N, K, act):
@@ -212,7 +231,8 @@ def experts_case(seed, rows, E, top, I, D, group, act, holes=True):
     (20, 3, 3, 136, 128, 128, (1.0, 0.0, 0.0)), (64, 4, 2, 64, 200, 32, (1.0, 0.0, 0.0)), (130, 2, 2, 48, 40, 64, (1.0, 0.0, 0.0)),
     (1, 5, 8, 136, 72, 32, (1.702, 7.0, 1.0)), (1, 4, 3, 20, 36, 64, (1.0, 0.0, 0.0)), (1, 3, 64, 24, 40, 32, (1.0, 0.0, 0.0)),
     (20, 16, 4, 72, 136, 32, (1.0, 0.0, 0.0)), (16, 2, 4, 40, 80, 64, (1.0, 0.0, 0.0)), (40, 64, 2, 16, 48, 32, (1.0, 0.0, 0.0)),
-    (150, 7, 2, 20, 36, 32, (1.702, 7.0, 1.0)), (3, 200, 8, 8, 16, 32, (1.0, 0.0, 0.0)), (400, 3, 2, 144, 264, 128, (1.0, 0.0, 0.0))])
+    (150, 7, 2, 20, 36, 32, (1.702, 7.0, 1.0)), (3, 200, 8, 8, 16, 32, (1.0, 0.0, 0.0)), (400, 3, 2, 144, 264, 128, (1.0, 0.0, 0.0)),
+    (1, 3, 2, 3, 5, 32, (1.0, 0.0, 0.0)), (4, 4, 2, 9, 3, 64, (1.0, 0.0, 0.0)), (60, 2, 2, 3, 13, 32, (1.0, 0.0, 0.0)), (2, 2, 2, 1, 1, 32, (1.0, 0.0, 0.0))])
 def test_experts(api, rows, E, top, I, D, group, act):
     fp4, ops = api
     gu, dn, x, ids, shares, exact, slack = experts_case(20, rows, E, top, I, D, group, act)
