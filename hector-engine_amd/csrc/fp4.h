@@ -56,6 +56,7 @@ struct Fp4Case {
   int bias_dtype;
   int M;
   GatedAct act;
+  bool silu;                  // act is plain silu
   const int32_t* ids;         // [choices]: an expert each (fewer than groups, or none); a choice's row is choice / top, its results row `choice`. Or null
   const float* shares;        // [choices]: one of zero is left out
   int choices, top;
@@ -69,64 +70,79 @@ struct Fp4Case {
 
 // The gated activation for results of 8 bits: the hardware's power of two and reciprocal, off by a few last places of 32-bit numbers
 // (2^-22 of the value, and 2^-24 |alpha gate| where the power's argument is rounded), in a third of the instructions of the library's
-// exponential and a division.
+// exponential and a division. NaN stays NaN behind the limits too. SILU: the constants are silu's, which takes half the instructions.
+template <bool SILU>
 __device__ __forceinline__ float fp4_act(float g, float u, const GatedAct& a) {
-  g = fminf(g, a.limit);
-  u = fminf(fmaxf(u, -a.limit), a.limit);
+  if (SILU) return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g)) * u;
+  g = g > a.limit ? a.limit : g;
+  u = u > a.limit ? a.limit : u < -a.limit ? -a.limit : u;
   const float z = fmaf(a.cubic, g * g, a.alpha) * g;
   return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z)) * (u + a.shift);
 }
 
-// a lane's four neighbouring results, columns n to n + 3 of row `to`, times f
-__device__ __forceinline__ void fp4_store(const Fp4Case& c, fp4_f32x4 v, int64_t to, int n, float f) {
-  if (c.gated) {
+// the bias of columns n to n + 3
+__device__ __forceinline__ fp4_f32x4 fp4_bias(const Fp4Case& c, int n) {
+  fp4_f32x4 b;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = load_param(c.bias, min(n + e, c.w.N - 1), c.bias_dtype);
+  return b;
+}
+
+// a lane's four neighbouring results, columns n to n + 3 of row `to`, whole: in one store; f: what activations are multiplied by
+enum { FP4_GATED, FP4_SILU, FP4_BF16, FP4_F32 };
+template <int KIND>
+__device__ __forceinline__ void fp4_put(const Fp4Case& c, fp4_f32x4 v, int64_t to, int n, float f, bool whole) {
+  if constexpr (KIND == FP4_GATED || KIND == FP4_SILU) {
     uint16_t* p = (uint16_t*)c.out + to * c.ldo + n / 2;
     auto act = [&](float g, float u) {
-      return f == 0.f ? 0.f : fp4_act(g, u, c.act) * f;    // (a choice without weight adds nothing, whatever its row holds)
+      return f == 0.f ? 0.f : fp4_act<KIND == FP4_SILU>(g, u, c.act) * f;    // (a choice without weight adds nothing, whatever its row holds)
     };
     const uint32_t pair = pack2_bf16(act(v[0], v[1]), act(v[2], v[3]));
-    if (c.pairs && n + 4 <= c.w.N) {
+    if (whole) {
       *reinterpret_cast<uint32_t*>(p) = pair;
     } else {
       p[0] = (uint16_t)pair;
       if (n + 2 < c.w.N) p[1] = (uint16_t)(pair >> 16);
     }
-    return;
-  }
-  if (c.bias)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += load_param(c.bias, min(n + e, c.w.N - 1), c.bias_dtype);
-  if (c.out_f32) {
+  } else if constexpr (KIND == FP4_F32) {
     float* p = (float*)c.out + to * c.ldo + n;
-    if (c.pairs && n + 4 <= c.w.N) {
+    if (whole) {
       *reinterpret_cast<fp4_f32x4*>(p) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (n + e < c.w.N) p[e] = v[e];
     }
-    return;
-  }
-  uint16_t* p = (uint16_t*)c.out + to * c.ldo + n;
-  const uint32_t a = pack2_bf16(v[0], v[1]), b = pack2_bf16(v[2], v[3]);
-  if (c.pairs && n + 4 <= c.w.N) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
   } else {
+    uint16_t* p = (uint16_t*)c.out + to * c.ldo + n;
+    const uint32_t a = pack2_bf16(v[0], v[1]), b = pack2_bf16(v[2], v[3]);
+    if (whole) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < c.w.N) p[e] = (uint16_t)((e < 2 ? a : b) >> (16 * (e & 1)));
+      for (int e = 0; e < 4; ++e)
+        if (n + e < c.w.N) p[e] = (uint16_t)((e < 2 ? a : b) >> (16 * (e & 1)));
+    }
   }
 }
+__device__ __forceinline__ void fp4_store(const Fp4Case& c, fp4_f32x4 v, int64_t to, int n, float f) {
+  const bool whole = c.pairs && n + 4 <= c.w.N;
+  if (c.gated && c.silu) return fp4_put<FP4_SILU>(c, v, to, n, f, whole);
+  if (c.gated) return fp4_put<FP4_GATED>(c, v, to, n, f, whole);
+  if (c.bias) v += fp4_bias(c, n);
+  if (c.out_f32) fp4_put<FP4_F32>(c, v, to, n, f, whole);
+  else fp4_put<FP4_BF16>(c, v, to, n, f, whole);
+}
 
-// the group of rows that tile `tile` belongs to: the last one that begins at or before it
+// the group of rows that tile `tile` belongs to, the last one that begins at or before it: the groups behind the first that do
+// (64 are looked at in one load; a search of halves waited for each of its loads)
 __device__ __forceinline__ int fp4_group_of(const int32_t* tile_begin, int groups, int tile) {
-  int lo = 0, hi = groups;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (tile_begin[mid] <= tile) lo = mid;
-    else hi = mid;
+  int group = 0;
+  for (int g = 1; g < groups; g += 64) {
+    const int mine = g + (int)(threadIdx.x & 63);
+    group += __popcll(__ballot(mine < groups && tile_begin[min(mine, groups)] <= tile));
   }
-  return lo;
+  return group;
 }
 
 // fp4_few.hip: rows in tiles of bm (4, 8 or 16); K is 8 at least

@@ -164,7 +164,7 @@ extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx
   c.x = (const uint16_t*)x, c.ldx = ldx, c.whole = whole_rows(x, ldx);
   c.out = out, c.ldo = ldo, c.out_f32 = out_dtype == HE_F32, c.gated = gated;
   c.bias = bias, c.bias_dtype = bias_dtype, c.M = M;
-  c.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic};
+  c.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic}, c.silu = he_gated_act_is_silu(alpha, limit, up_shift, cubic);
   c.pairs = ldo % (gated ? 2 : 4) == 0 && ((uintptr_t)out & (out_dtype == HE_F32 ? 15 : gated ? 3 : 7)) == 0;
   hipStream_t s = (hipStream_t)stream;
   const ProductScratch t = product_scratch(M, N, K, c.whole && !far(M, ldx));
@@ -210,7 +210,7 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
   float* partial = (float*)(p + t.ints + t.h);
   up.x = (const uint16_t*)x, up.ldx = ldx, up.whole = whole_rows(x, ldx), up.M = rows;
   up.out = h, up.ldo = t.ldh, up.pairs = t.ldh % 2 == 0, up.gated = true;
-  up.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic};
+  up.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic}, up.silu = he_gated_act_is_silu(alpha, limit, up_shift, cubic);
   up.tile_begin = lists.tile_begin, up.groups = experts, up.rows_of = lists.rows_of, up.out_of = lists.choice_of, up.factor = lists.scale;
   down.x = h, down.ldx = t.ldh, down.whole = true;
   down.out = partial, down.ldo = D, down.out_f32 = true, down.pairs = D % 4 == 0;

@@ -27,6 +27,8 @@ __global__ __launch_bounds__(256, 2) void fp4_tall_kernel(Fp4Case c, int mtiles,
   constexpr int RING = 16 / NT < 4 * MT ? 16 / NT : 4 * MT;                // operands of X in registers: some 250 cycles of products
   constexpr int FEW = MT < 4 ? MT : 4, ROW = 64 * NT + 16, TURN = 16 * FEW * ROW;      // results: tiles of rows a turn; bytes of a row, a wavefront's turn
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BLOCK > 4 * TURN ? 2 * BLOCK : 4 * TURN];
+  __shared__ int32_t to_of[BM];                            // a slot's row of out, -1: none
+  __shared__ float share_of[BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
   // tiles of rows that read the same weights are neighbours on an XCD
   const int per_xcd = gridDim.x / HE_XCDS;
@@ -91,6 +93,11 @@ __global__ __launch_bounds__(256, 2) void fp4_tall_kernel(Fp4Case c, int mtiles,
   fetch_w(lo);
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) fetch_x(l, lo, 0);
+  if (tid < BM) {
+    const int slot = m0 + tid;
+    to_of[tid] = c.out_of ? c.out_of[slot] : slot < c.M ? slot : -1;
+    share_of[tid] = c.factor ? c.factor[slot] : 1.f;
+  }
   uint32_t at = 0;
   for (int kb = lo; kb < hi; ++kb) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -143,24 +150,41 @@ __global__ __launch_bounds__(256, 2) void fp4_tall_kernel(Fp4Case c, int mtiles,
   // some tiles of rows at a time through this wavefront's part of LDS, so that neighbouring lanes write neighbouring results
   uint8_t* own = lds + wave * TURN;
   const int n = tile0 * FP4_ROWS + lane % (4 * NT) * 4, ld_parts = c.w.tiles * FP4_ROWS;
+  const bool whole = c.pairs && n + 4 <= c.w.N;
+  fp4_f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+  if (c.bias) bias = fp4_bias(c, n);
 #pragma unroll
   for (int i0 = 0; i0 < MT; i0 += FEW) {
 #pragma unroll
     for (int i = i0; i < i0 + FEW; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) *reinterpret_cast<fp4_f32x4*>(own + (16 * (i - i0) + r16) * ROW + (16 * j + 4 * kq) * 4) = acc[i][j];
+    // (one kind of results a loop: with the kinds told apart at each of them 128 x 256 results of K 2048 took 1.1 of the time)
+    auto rows = [&](auto put) {
 #pragma unroll 4
-    for (int r = lane / (4 * NT); r < 16 * FEW; r += 16 / NT) {
-      const int slot = m0 + 16 * i0 + r;
-      const fp4_f32x4 v = *reinterpret_cast<const fp4_f32x4*>(own + r * ROW + lane % (4 * NT) * 16);
-      if (slices > 1) {
-        if (slot < c.M && n < ld_parts) *reinterpret_cast<fp4_f32x4*>(parts + ((int64_t)slice * c.M + slot) * ld_parts + n) = v;
-        continue;
-      }
-      int to = slot;
-      if (c.out_of) to = c.out_of[slot];
-      else if (slot >= c.M) to = -1;
-      if (to >= 0 && n < c.w.N) fp4_store(c, v, to, n, c.factor ? c.factor[slot] : 1.f);
+      for (int r = lane / (4 * NT); r < 16 * FEW; r += 16 / NT)
+        put(16 * i0 + r, *reinterpret_cast<const fp4_f32x4*>(own + r * ROW + lane % (4 * NT) * 16));
+    };
+    if (slices > 1) {
+      rows([&](int r, fp4_f32x4 v) {
+        if (to_of[r] >= 0 && n < ld_parts) *reinterpret_cast<fp4_f32x4*>(parts + ((int64_t)slice * c.M + m0 + r) * ld_parts + n) = v;
+      });
+    } else if (c.gated && c.silu) {
+      rows([&](int r, fp4_f32x4 v) {
+        if (to_of[r] >= 0 && n < c.w.N) fp4_put<FP4_SILU>(c, v, to_of[r], n, share_of[r], whole);
+      });
+    } else if (c.gated) {
+      rows([&](int r, fp4_f32x4 v) {
+        if (to_of[r] >= 0 && n < c.w.N) fp4_put<FP4_GATED>(c, v, to_of[r], n, share_of[r], whole);
+      });
+    } else if (c.out_f32) {
+      rows([&](int r, fp4_f32x4 v) {
+        if (to_of[r] >= 0 && n < c.w.N) fp4_put<FP4_F32>(c, v + bias, to_of[r], n, 1.f, whole);
+      });
+    } else {
+      rows([&](int r, fp4_f32x4 v) {
+        if (to_of[r] >= 0 && n < c.w.N) fp4_put<FP4_BF16>(c, v + bias, to_of[r], n, 1.f, whole);
+      });
     }
   }
 }

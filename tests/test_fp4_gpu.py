@@ -195,6 +195,10 @@ def test_a_row_without_numbers_stays_alone(api):
         keep[1:3], keep[:, 7] = False, False
         assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
         assert got[1].isnan().all() and got[:, 7].isnan().all() and not got[2].isfinite().any()
+        for act in ((1.0, 0.0, 0.0), (1.702, 7.0, 1.0), (1.5957691216057308, 0.0, 0.0, 0.07135481627159956)):      # (limits do not hide a NaN)
+            h = torch.empty((M, 20), dtype=BF16, device="cuda")
+            ops.fp4_product(h, x.cuda(), fp4.pack(w.cuda(), 64), None, M, gated=True, act=act, workspace=size)
+            assert h[1].isnan().all() and h[:, 3].isnan().all() and h.cpu()[keep[:, 0::2] & keep[:, 1::2]].isfinite().all()
 
 
 def experts_case(seed, rows, E, top, I, D, group, act, holes=True):
