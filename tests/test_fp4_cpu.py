@@ -1,0 +1,116 @@
+"""Weights in 4 bits without a GPU: the layout's sizes, the definition, the operators' refusals and their choices by size."""
+import ctypes
+
+import pytest
+import torch
+
+from tests.plain import fp4_plain as P
+
+F64 = torch.float64
+
+
+@pytest.fixture(scope="module")
+def L():
+    from hector_engine_amd.kernels import lib
+    return lib.load()
+
+
+def refusal(L, status):
+    assert status != 0
+    return L.he_last_error().decode()
+
+
+ROOM = ctypes.create_string_buffer(4096)
+AT = (ctypes.addressof(ROOM) + 255) // 256 * 256       # (an address: no call of this file launches anything)
+
+
+@pytest.mark.parametrize("shape,group,codes,scales", [
+    ((16, 128), 32, (1, 1, 1024), (1, 1, 4, 16)), ((17, 129), 64, (2, 2, 1024), (2, 2, 2, 16)), ((1, 1), 128, (1, 1, 1024), (1, 1, 1, 16)),
+    ((3, 40, 300), 128, (3, 3, 3, 1024), (3, 3, 3, 1, 16))])
+def test_sizes_of_the_layout(shape, group, codes, scales):
+    from hector_engine_amd.kernels import fp4
+    assert fp4.storage_shapes(shape, group) == (codes, scales)
+
+
+def test_refusals_of_packing():
+    from hector_engine_amd.kernels import fp4
+    for shape in ((4,), (0, 4), (4, 0), (2, 3, 4, 5)):
+        with pytest.raises(ValueError, match="positive sizes"):
+            fp4.storage_shapes(shape, 64)
+    for group in (0, 16, 48, 256):
+        with pytest.raises(ValueError, match=f"groups of {group}"):
+            fp4.storage_shapes((4, 4), group)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        fp4.pack(torch.zeros(4, 64))
+    with pytest.raises(ValueError, match="one GPU"):
+        fp4.Fp4Weight(torch.zeros(1, 1, 1024, dtype=torch.uint8), torch.zeros(1, 1, 2, 16, dtype=torch.bfloat16), (4, 64), 64)
+
+
+def test_the_definition_keeps_what_it_says():
+    """Values that packing gives are bfloat16 numbers; the largest of a group is off by a sixty-fourth at most, no value by more than a
+    sixth of it and that; packing them again gives them again."""
+    w = torch.randn(50, 300, generator=torch.Generator().manual_seed(1), dtype=F64)
+    w[3, 64:128] = 0
+    for group in (32, 64, 128):
+        v = P.values(w, group)
+        assert torch.equal(v.to(torch.bfloat16).double(), v) and (v[3, 64:96] == 0).all()
+        for k0 in range(0, 300, group):
+            a, b = w[:, k0:k0 + group], v[:, k0:k0 + group]
+            most = a.abs().amax(-1, keepdim=True)
+            at = a.abs() == most
+            assert ((a - b).abs()[at] <= most.expand_as(a)[at] / 64).all()
+            assert ((a - b).abs() <= most * (1 / 6 + 1 / 64)).all()
+        assert torch.equal(P.values(v, group), v)
+
+
+def test_refusals_of_the_product(L):
+    def call(M=4, N=32, K=64, ldo=32, ldx=64, codes=AT, scales=AT, bias=None, group=32, out_dtype=0, gated=0, workspace=None, size=0):
+        return refusal(L, L.he_fp4_product(AT, ldo, AT, ldx, codes, scales, bias, M, N, K, group, out_dtype, 0, gated, 1.0, 0.0, 0.0, 0.0, workspace, size, None))
+    assert "groups of 48" in call(group=48)
+    assert "a weight of [0, 64]" in call(N=0)
+    assert "16-byte aligned" in call(codes=AT + 8) and "16-byte aligned" in call(codes=None) and "16-byte aligned" in call(scales=AT + 2)
+    assert "rows of 64 at distances" in call(M=-1) and "rows of 64 at distances" in call(ldx=63) and "rows of 64 at distances" in call(ldo=31)
+    assert "rows of 64 at distances" in call(M=(1 << 22) + 1)
+    assert "dtype code 7" in call(out_dtype=7)
+    assert "gated" in call(gated=1, out_dtype=0) and "gated" in call(gated=1, out_dtype=1, bias=AT) and "gated" in call(gated=1, out_dtype=1, N=33)
+    need = L.he_fp4_product_workspace_bytes(3, 32, 5, 1)
+    assert need > 0 and "a workspace of" in call(M=3, K=5) and "a workspace of" in call(M=3, K=5, workspace=AT, size=need - 1) \
+        and "a workspace of" in call(M=3, K=5, workspace=AT + 8, size=need)
+
+
+def test_refusals_of_the_experts(L):
+    def call(rows=4, top=2, experts=2, I=16, D=64, ldx=64, up=AT, down=AT, groups=(32, 32), workspace=AT, size=1 << 30):
+        return refusal(L, L.he_fp4_experts(AT, AT, ldx, up, AT, down, AT, AT, AT, rows, top, experts, I, D, *groups, 0, 1.0, 0.0, 0.0, 0.0, workspace, size, None))
+    assert "bad sizes" in call(rows=-1) and "bad sizes" in call(top=0) and "bad sizes" in call(I=0) and "bad sizes" in call(D=0) and "bad sizes" in call(experts=0)
+    assert "too many" in call(experts=1025) and "too many" in call(rows=65536) and "too many" in call(rows=65535, top=4096)
+    assert "distance of 63" in call(ldx=63)
+    assert "groups of 16" in call(groups=(16, 32)) and "groups of 256" in call(groups=(32, 256))
+    assert "16-byte aligned" in call(up=AT + 4) and "16-byte aligned" in call(down=None)
+    need = L.he_fp4_experts_workspace_bytes(4, 2, 2, 16, 64)
+    assert need > 0 and "a workspace of" in call(workspace=None) and "a workspace of" in call(size=need - 1) and "a workspace of" in call(workspace=AT + 4)
+
+
+def test_no_rows_want_nothing(L):
+    assert L.he_fp4_product_workspace_bytes(0, 32, 64, 1) == 0 and L.he_fp4_experts_workspace_bytes(0, 2, 2, 16, 64) == 0
+    assert L.he_fp4_product(AT, 32, AT, 64, AT, AT, None, 0, 32, 64, 32, 0, 0, 0, 1.0, 0.0, 0.0, 0.0, None, 0, None) == 0
+    assert L.he_fp4_experts(AT, AT, 64, AT, AT, AT, AT, AT, AT, 0, 2, 2, 16, 64, 32, 32, 0, 1.0, 0.0, 0.0, 0.0, None, 0, None) == 0
+
+
+def test_which_products_want_a_workspace(L):
+    """Few rows, and small weights, are read as they are wherever they lie; larger products copy rows that are not whole blocks of 128
+    values or lie at odd places, and keep the sums of slices of K."""
+    def wants(M, N, K, whole=1):
+        return L.he_fp4_product_workspace_bytes(M, N, K, whole)
+    for M in (1, 8, 16):
+        assert wants(M, 37888, 3584, 0) == wants(M, 1001, 1003, 0) == 0
+    assert wants(64, 1001, 1003, 0) == wants(128, 512, 896, 0) == 0
+    assert wants(2048, 37888, 3584) == 0 and wants(2048, 37888, 3584, 0) == 2048 * 3584 * 2
+    assert wants(2048, 37888, 3590) == wants(2048, 37888, 3590, 0) == 2048 * 3712 * 2
+    slices = wants(64, 3584, 18944) / (64 * 3584 * 4)
+    assert slices in (2, 4, 8, 16)
+
+
+def test_the_route_of_packed_weights():
+    from hector_engine_amd.kernels import routes
+    import hector_engine_amd.parts.linear  # noqa: F401
+    assert [r.name for r in routes.routes_of("linear", ("fp4", torch.bfloat16))] == ["fp4"]
