@@ -65,6 +65,15 @@ struct Fp4Case {
   const int32_t* rows_of;     // a slot's row of x, -1: none
   const int32_t* out_of;      // a slot's row of out, -1: none
   const float* factor;        // what a slot's (with ids: a choice's) results are multiplied by, or null
+  const float* owed;          // [M][owed_count], or null: the sums over row m times 1 / sqrt(the sum of owed[m] / owed_dim + owed_eps), x's rows being a norm's without its scale
+  int owed_count, owed_dim;
+  float owed_eps;
+  float* resid;               // [M][N], or null: in place of out, resid += resid_scale * result, carried = bf16(resid * gain), squares[m][tile] = the
+  float resid_scale;          // tile's sum of resid^2 (fp4_few.hip alone, N a multiple of 4)
+  const void* gain;
+  int gain_dtype;
+  uint16_t* carried;
+  float* squares;
   bool pairs;                 // out takes stores of four neighbouring results (gated: of two)
 };
 

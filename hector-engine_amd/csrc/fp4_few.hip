@@ -8,20 +8,26 @@ struct __attribute__((packed, aligned(2))) Piece {
   uint4 v;
 };
 
+enum { ROWS_ALONE, CHOICES, NORM };
+
 // A workgroup has NT tiles of 16 weight rows; its W wavefronts cut K among them, and their sums meet in LDS. Codes, scales and X (4 XL rows of it)
 // come straight into registers, D blocks of 128 k ahead, with no barrier before the end. A block of X goes from there through a
 // wavefront's own part of LDS into the order of the operands: read as operands from memory, each of its rows a sixteen-byte piece a
 // lane and all 16 of them whatever X has, it took a third of the time (8 rows of 37888 x 3584 19.5 us, without it 14).
 // There the pieces of a row lie at their index xor the row, so that the rows of an operand are in different banks.
 // With ids (64 choices at most) a tile's slots are found here, by every wavefront for itself: slot by slot the choices of one expert, the
-// tiles in the order of their first choices. CHAIN: one row and all of its choices, a tile's sums taken over the choices' K one after the
+// tiles in the order of their first choices. CHOICES: one row and all of its choices, a tile's sums taken over the choices' K one after the
 // other (codes of expert ids[choice], X row `choice`), so that nothing is left to add up.
-template <int NT, int W, int D, int XL, int GROUPS, bool CHAIN>
+// NORM: a norm is carried across two products (resid, owed): the first adds its results to the residual rows and leaves r * gain and the sums of
+// r^2, the second multiplies its sums by the row's scale, whose parts are read, all at once, while its first codes are on their way.
+template <int NT, int W, int D, int XL, int GROUPS, int KIND>
 __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[W * (NT > 2 * XL ? NT : 2 * XL) * 1024];
+  constexpr bool CHAIN = KIND == CHOICES, CARRIED = KIND == NORM;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
   constexpr int ROWS = 4 * XL;                             // of a tile of rows
   __shared__ int32_t choice_in[W][16];                     // with ids: a slot's choice, -1: none
+  __shared__ float scale_of[16];                           // with owed: a row's scale
   const int blocks = c.w.blocks, units = CHAIN ? c.choices * blocks : blocks;      // (a unit: a block of a choice)
   const int lo = units * wave / W, hi = units * (wave + 1) / W;
   int group = 0;
@@ -132,6 +138,33 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   if (lo < hi) {
 #pragma unroll
     for (int u = 0; u < D; ++u) load(u, min(lo + u, hi - 1));
+  }
+  if (CARRIED && c.owed) {
+    constexpr int EACH = (ROWS + W - 1) / W;               // rows of a wavefront
+    float sum[EACH];
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) sum[r] = 0.f;
+    for (int from = 0; from < c.owed_count; from += 256) {
+      float part[EACH][4];
+#pragma unroll
+      for (int r = 0; r < EACH; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = min(wave + r * W, c.M - 1), at = from + 64 * i + lane;
+          part[r][i] = c.owed[(int64_t)row * c.owed_count + min(at, c.owed_count - 1)];
+        }
+#pragma unroll
+      for (int r = 0; r < EACH; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[r] += from + 64 * i + lane < c.owed_count ? part[r][i] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      const float total = wave_sum(sum[r]);
+      if (lane == 0 && wave + r * W < ROWS) scale_of[wave + r * W] = 1.f / sqrtf(total / (float)c.owed_dim + c.owed_eps);
+    }
+  }
+  if (lo < hi) {
     int kb = lo;
     for (; kb + D < hi; kb += D) {
 #pragma unroll
@@ -159,27 +192,44 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   else if (c.ids) to = choice_in[wave][r16];
   else if (c.out_of) to = c.out_of[slot];
   else if (slot >= c.M) to = -1;
+  static_assert(NT <= W, "a wavefront has one tile of results");
+  if (wave >= NT) return;
+  const int n = (tile0 + wave) * FP4_ROWS + 4 * kq;
+  fp4_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    if (j % W != wave) continue;
-    fp4_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < W; ++k) v += *reinterpret_cast<const fp4_f32x4*>(lds + (k * NT + wave) * 1024 + lane * 16);
+  if (CARRIED && c.owed && to >= 0) v *= scale_of[r16];
+  if (CARRIED && c.resid) {
+    // (read ahead of the products they cost every kernel that carries a norm more than they saved this one)
+    float square = 0.f;
+    if (to >= 0 && n < c.w.N) {
+      if (c.bias) v += fp4_bias(c, n);
+      fp4_f32x4* r = reinterpret_cast<fp4_f32x4*>(c.resid + (int64_t)to * c.w.N + n);
+      v = *r + c.resid_scale * v;
+      *r = v;
+      float g[4];
 #pragma unroll
-    for (int k = 0; k < W; ++k) v += *reinterpret_cast<const fp4_f32x4*>(lds + (k * NT + j) * 1024 + lane * 16);
-    const int n = (tile0 + j) * FP4_ROWS + 4 * kq;
-    if (to >= 0 && n < c.w.N) fp4_store(c, v, to, n, c.factor ? c.factor[c.ids ? to : slot] : 1.f);
+      for (int e = 0; e < 4; ++e) square = fmaf(v[e], v[e], square), g[e] = v[e] * load_param(c.gain, n + e, c.gain_dtype);
+      *reinterpret_cast<uint2*>(c.carried + (int64_t)to * c.w.N + n) = make_uint2(pack2_bf16(g[0], g[1]), pack2_bf16(g[2], g[3]));
+    }
+    square += __shfl_xor(square, 16);
+    square += __shfl_xor(square, 32);
+    if (kq == 0 && to >= 0 && n < c.w.N) c.squares[(int64_t)to * c.w.tiles + tile0 + wave] = square;
+    return;
   }
+  if (to >= 0 && n < c.w.N) fp4_store(c, v, to, n, c.factor ? c.factor[c.ids ? to : slot] : 1.f);
 }
 
-template <int NT, int W, int D, int XL, bool CHAIN = false>
+template <int NT, int W, int D, int XL, int KIND>
 int run_few(const Fp4Case& c, int mtiles, hipStream_t s) {
   const dim3 grid((c.w.tiles + NT - 1) / NT, mtiles);
-  if (c.w.group == 128) fp4_few_kernel<NT, W, D, XL, 1, CHAIN><<<grid, 64 * W, 0, s>>>(c);
-  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, XL, 2, CHAIN><<<grid, 64 * W, 0, s>>>(c);
-  else fp4_few_kernel<NT, W, D, XL, 4, CHAIN><<<grid, 64 * W, 0, s>>>(c);
+  if (c.w.group == 128) fp4_few_kernel<NT, W, D, XL, 1, KIND><<<grid, 64 * W, 0, s>>>(c);
+  else if (c.w.group == 64) fp4_few_kernel<NT, W, D, XL, 2, KIND><<<grid, 64 * W, 0, s>>>(c);
+  else fp4_few_kernel<NT, W, D, XL, 4, KIND><<<grid, 64 * W, 0, s>>>(c);
   return he_check_launch("he_fp4_product");
 }
 
-template <int XL>
+template <int XL, int KIND>
 int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
   // Microseconds of (tiles, wavefronts, blocks ahead) = (1, 8, 2), (1, 8, 4), (2, 4, 2), (2, 8, 2), (4, 4, 2), weights from memory:
   // 1 row of 4608 x 3584 5.0, 5.4, 5.5, 4.8, 7.0; 3584 x 18944 10.5, 9.3, 17.4, 12.4, 23.8; 5120 x 27648 19.8, 20.2, 25.0, 17.6, 33.5; 8 rows of
@@ -187,24 +237,28 @@ int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
   const int64_t tiles = (int64_t)c.w.tiles * mtiles;
   if (tiles <= 256) {
     if constexpr (XL == 1) {
-      if (c.w.blocks >= 64) return run_few<1, 8, 4, XL>(c, mtiles, s);
+      if (c.w.blocks >= 64) return run_few<1, 8, 4, XL, KIND>(c, mtiles, s);
     }
-    return run_few<1, 8, 2, XL>(c, mtiles, s);
+    return run_few<1, 8, 2, XL, KIND>(c, mtiles, s);
   }
-  if (XL == 4 && tiles >= 640) return run_few<4, 4, 2, XL>(c, mtiles, s);
-  return tiles <= 512 && c.w.blocks >= 64 ? run_few<2, 8, 2, XL>(c, mtiles, s) : run_few<2, 4, 2, XL>(c, mtiles, s);
+  if (XL == 4 && tiles >= 640) return run_few<4, 4, 2, XL, KIND>(c, mtiles, s);
+  return tiles <= 512 && c.w.blocks >= 64 ? run_few<2, 8, 2, XL, KIND>(c, mtiles, s) : run_few<2, 4, 2, XL, KIND>(c, mtiles, s);
 }
 
 }  // namespace
 
 int fp4_run_chain(const Fp4Case& c, hipStream_t s) {
   HE_REQUIRE(c.w.K >= 8 && c.ids && c.choices >= 1 && c.choices <= 64 && c.M == 1, "he_fp4_experts: %d choices of a row", c.choices);
-  return c.w.tiles <= 256 ? run_few<1, 8, 2, 1, true>(c, 1, s) : run_few<2, 8, 2, 1, true>(c, 1, s);
+  return c.w.tiles <= 256 ? run_few<1, 8, 2, 1, CHOICES>(c, 1, s) : run_few<2, 8, 2, 1, CHOICES>(c, 1, s);
 }
 
 int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s) {
   HE_REQUIRE(c.w.K >= 8, "he_fp4_product: rows of fewer than 8 values");
   HE_REQUIRE(!c.ids || c.choices <= 64, "he_fp4_experts: %d choices to be grouped by each workgroup", c.choices);
   HE_REQUIRE(mtiles <= 65535, "he_fp4_product: %d tiles of rows are too many for one launch", mtiles);
-  return bm > 8 ? run_rows<4>(c, mtiles, s) : bm > 4 ? run_rows<2>(c, mtiles, s) : run_rows<1>(c, mtiles, s);
+  if (c.owed || c.resid) {
+    HE_REQUIRE(mtiles == 1 && !c.ids && !c.tile_begin, "he_fp4_product: a norm is carried by one tile of rows");
+    return bm > 8 ? run_rows<4, NORM>(c, 1, s) : bm > 4 ? run_rows<2, NORM>(c, 1, s) : run_rows<1, NORM>(c, 1, s);
+  }
+  return bm > 8 ? run_rows<4, ROWS_ALONE>(c, mtiles, s) : bm > 4 ? run_rows<2, ROWS_ALONE>(c, mtiles, s) : run_rows<1, ROWS_ALONE>(c, mtiles, s);
 }

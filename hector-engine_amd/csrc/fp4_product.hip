@@ -151,21 +151,35 @@ extern "C" int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int whole
   return M <= 0 || N <= 0 || K <= 0 ? 0 : product_scratch(M, N, K, whole).bytes;
 }
 
+// the case of he_fp4_product without its results
+static int product_case(Fp4Case* c, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M, int N, int K, int group,
+                        int bias_dtype) {
+  *c = {};
+  c->w = weight(codes, scales, N, K, group);
+  if (const int rc = check_weight("he_fp4_product", c->w)) return rc;
+  HE_REQUIRE(M >= 0 && M <= (1 << 22) && ldx >= K, "he_fp4_product: %d rows of %d at distances of %lld", M, K, (long long)ldx);
+  c->x = (const uint16_t*)x, c->ldx = ldx, c->whole = whole_rows(x, ldx), c->M = M, c->bias = bias, c->bias_dtype = bias_dtype;
+  return 0;
+}
+
+static void results(Fp4Case* c, void* out, int64_t ldo, int out_dtype, int gated, GatedAct act) {
+  c->out = out, c->ldo = ldo, c->out_f32 = out_dtype == HE_F32, c->gated = gated;
+  c->silu = he_gated_act_is_silu(act.alpha, act.limit, act.shift, act.cubic);
+  c->act = act;
+  if (!(act.limit > 0.f)) c->act.limit = INFINITY;
+  c->pairs = ldo % (gated ? 2 : 4) == 0 && ((uintptr_t)out & (out_dtype == HE_F32 ? 15 : gated ? 3 : 7)) == 0;
+}
+
 extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M, int N,
                               int K, int group, int out_dtype, int bias_dtype, int gated, float alpha, float limit, float up_shift, float cubic,
                               void* workspace, int64_t workspace_bytes, void* stream) {
-  Fp4Case c = {};
-  c.w = weight(codes, scales, N, K, group);
-  if (const int rc = check_weight("he_fp4_product", c.w)) return rc;
-  HE_REQUIRE(M >= 0 && M <= (1 << 22) && ldx >= K && ldo >= (gated ? N / 2 : N), "he_fp4_product: %d rows of %d at distances %lld and %lld", M, K, (long long)ldx, (long long)ldo);
+  Fp4Case c;
+  if (const int rc = product_case(&c, x, ldx, codes, scales, bias, M, N, K, group, bias_dtype)) return rc;
+  HE_REQUIRE(ldo >= (gated ? N / 2 : N), "he_fp4_product: results of %d at distances of %lld", gated ? N / 2 : N, (long long)ldo);
   HE_REQUIRE(out_dtype == HE_F32 || out_dtype == HE_BF16, "he_fp4_product: dtype code %d", out_dtype);
   HE_REQUIRE(!gated || (N % 2 == 0 && out_dtype == HE_BF16 && !bias), "he_fp4_product: a gated product has an even N, bfloat16 results and no bias");
   if (M == 0) return 0;
-  c.x = (const uint16_t*)x, c.ldx = ldx, c.whole = whole_rows(x, ldx);
-  c.out = out, c.ldo = ldo, c.out_f32 = out_dtype == HE_F32, c.gated = gated;
-  c.bias = bias, c.bias_dtype = bias_dtype, c.M = M;
-  c.act = {alpha, limit > 0.f ? limit : INFINITY, up_shift, cubic}, c.silu = he_gated_act_is_silu(alpha, limit, up_shift, cubic);
-  c.pairs = ldo % (gated ? 2 : 4) == 0 && ((uintptr_t)out & (out_dtype == HE_F32 ? 15 : gated ? 3 : 7)) == 0;
+  results(&c, out, ldo, out_dtype, gated, {alpha, limit, up_shift, cubic});
   hipStream_t s = (hipStream_t)stream;
   const ProductScratch t = product_scratch(M, N, K, c.whole && !far(M, ldx));
   HE_REQUIRE(t.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= t.bytes),
@@ -174,6 +188,28 @@ extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx
     if (const int rc = pad_rows(&c, workspace, s)) return rc;
   if (t.plan.mt == 0) return fp4_run_few(c, M > 8 ? 16 : M > 4 ? 8 : 4, (M + 15) / 16, s);
   return fp4_run_tall(c, t.plan, (M + 16 * t.plan.mt - 1) / (16 * t.plan.mt), (float*)((uint8_t*)workspace + t.rows), s);
+}
+
+extern "C" int he_fp4_product_carried(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M,
+                                      int N, int K, int group, int out_dtype, int bias_dtype, int gated, float alpha, float limit, float up_shift, float cubic,
+                                      const void* owed, int owed_count, float owed_eps, void* resid, float resid_scale, const void* gain, int gain_dtype,
+                                      void* carried, void* squares, void* stream) {
+  Fp4Case c;
+  if (const int rc = product_case(&c, x, ldx, codes, scales, bias, M, N, K, group, bias_dtype)) return rc;
+  HE_REQUIRE(M <= 16 && K >= 8, "he_fp4_product_carried: %d rows of %d (up to 16, of 8 or more)", M, K);
+  HE_REQUIRE(!owed || owed_count > 0, "he_fp4_product_carried: %d sums of squares a row", owed_count);
+  if (resid) {
+    HE_REQUIRE(N % 4 == 0 && !gated && !out && gain && carried && squares && (((uintptr_t)resid & 15) | ((uintptr_t)carried & 7)) == 0,
+               "he_fp4_product_carried: results for the residual rows are not gated, N is a multiple of 4, their buffers are there and aligned");
+  } else {
+    HE_REQUIRE(out && ldo >= (gated ? N / 2 : N) && (out_dtype == HE_F32 || out_dtype == HE_BF16), "he_fp4_product_carried: results of dtype code %d at distances of %lld", out_dtype, (long long)ldo);
+    HE_REQUIRE(!gated || (N % 2 == 0 && out_dtype == HE_BF16 && !bias), "he_fp4_product_carried: a gated product has an even N, bfloat16 results and no bias");
+  }
+  if (M == 0) return 0;
+  results(&c, out, ldo, out_dtype, gated, {alpha, limit, up_shift, cubic});
+  c.owed = (const float*)owed, c.owed_count = owed_count, c.owed_dim = K, c.owed_eps = owed_eps;
+  c.resid = (float*)resid, c.resid_scale = resid_scale, c.gain = gain, c.gain_dtype = gain_dtype, c.carried = (uint16_t*)carried, c.squares = (float*)squares;
+  return fp4_run_few(c, M > 8 ? 16 : M > 4 ? 8 : 4, 1, (hipStream_t)stream);
 }
 
 extern "C" int64_t he_fp4_experts_workspace_bytes(int rows, int top, int experts, int I, int D) {

@@ -462,6 +462,13 @@ int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int whole);
 int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M, int N,
                    int K, int group, int out_dtype, int bias_dtype, int gated, float alpha, float limit, float up_shift, float cubic,
                    void* workspace, int64_t workspace_bytes, void* stream);
+// The product of up to 16 rows that a norm is carried across (K 8 at least). owed: the sums over row m are multiplied by 1 / sqrt(the sum of
+// owed[m][owed_count] / K + owed_eps). resid (out null): resid[M][N] += resid_scale * result, carried[M][N] = bf16(resid * gain), squares[M][N / 16, rounded up] =
+// the sums of resid^2 over 16 columns.
+int he_fp4_product_carried(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M, int N,
+                           int K, int group, int out_dtype, int bias_dtype, int gated, float alpha, float limit, float up_shift, float cubic,
+                           const void* owed, int owed_count, float owed_eps, void* resid, float resid_scale, const void* gain, int gain_dtype,
+                           void* carried, void* squares, void* stream);
 // A routed feed-forward over packed experts: out[row] (bf16 [rows][D]) = the sum over the row's choices (ids [rows][top], the expert; an id
 // that is none adds nothing, with identity one from `experts` on weights x) of weights[row][choice] * down_e act(gate_e x, up_e x). up: matrices of [2 I, D], gate and up rows in
 // turn; down: matrices of [D, I].

@@ -121,6 +121,8 @@ _SIGNATURES = {
     "he_fp4_product_workspace_bytes": [c_int, c_int, c_int, c_int],
     "he_fp4_product": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32,
                        c_f32, c_f32, c_ptr, c_i64, c_ptr],
+    "he_fp4_product_carried": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32,
+                               c_f32, c_f32, c_ptr, c_int, c_f32, c_ptr, c_f32, c_ptr, c_int, c_ptr, c_ptr, c_ptr],
     "he_fp4_experts_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
     "he_fp4_experts": [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                        c_f32, c_f32, c_f32, c_f32, c_ptr, c_i64, c_ptr],

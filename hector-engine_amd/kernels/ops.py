@@ -1499,6 +1499,57 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.
                                 dtype_code(dtype), F32 if bias is None else dtype_code(bias.dtype), gated, *_act4(act), ws, size, _stream()))
 
 
+FP4_CARRIED_ROWS = 16
+
+
+@_op("fp4_product")
+def fp4_product_carried(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.0, 0.0), row_scale=None, residual=None) -> None:
+    """fp4_product of up to 16 rows (K 8 at least) that an RMS norm is carried across. row_scale = (partials float32 [rows or more, count], eps): the rows of
+    x are r * gain of a norm whose 1 / sqrt(mean(r^2) + eps) is applied to the sums here (mean over K). residual = (resid float32 [rows or more, N],
+    gain [N], xg bfloat16, squares float32 [rows or more, ceil(N / 16)][, scale]): instead of writing `out` (None), resid += scale * result in place,
+    xg = resid * gain, squares = the sums of resid^2 over sixteen columns (N a multiple of 4)."""
+    device = _fp4_weight("fp4_product_carried", w, 2)
+    N, K = w.shape
+    if not 0 <= rows <= FP4_CARRIED_ROWS or K < 8:
+        raise ValueError(f"fp4_product_carried: {rows} rows of {K}, it takes up to {FP4_CARRIED_ROWS} of 8 values or more")
+    if gated and (N % 2 or bias is not None):
+        raise ValueError("fp4_product_carried: a gated product has an even number of weight rows and no bias")
+    ldx = _fp4_rows("fp4_product_carried", "x", x, rows, K, torch.bfloat16, device)
+    if bias is not None:
+        _need(bias, "fp4_product_carried: bias", shape=(N,))
+        _fp4_on("fp4_product_carried", "bias", bias, device)
+    owed, count, eps = None, 0, 0.0
+    if row_scale is not None:
+        partials, eps = row_scale
+        _need(partials, "fp4_product_carried: row_scale", torch.float32)
+        _fp4_on("fp4_product_carried", "row_scale", partials, device)
+        if partials.dim() != 2 or partials.shape[0] < rows or partials.shape[1] == 0:
+            raise ValueError(f"fp4_product_carried: row_scale{tuple(partials.shape)} is not [{rows}, count]")
+        owed, count = partials.data_ptr(), partials.shape[1]
+    ldo, dtype, resid = N, torch.bfloat16, (None, 1.0, None, F32, None, None)
+    if residual is not None:
+        r, gain, xg, squares, *scale = residual
+        if out is not None or gated or N % 4:
+            raise ValueError("fp4_product_carried: results for the residual rows are no output and not gated, N is a multiple of 4")
+        for what, t, kind, cols in (("resid", r, torch.float32, N), ("xg", xg, torch.bfloat16, N), ("squares", squares, torch.float32, -(-N // 16))):
+            _need(t, f"fp4_product_carried: {what}")
+            if _fp4_rows("fp4_product_carried", what, t, rows, cols, kind, device) != cols:
+                raise ValueError(f"fp4_product_carried: {what}'s rows must lie together")
+        _need(gain, "fp4_product_carried: gain", shape=(N,))
+        _fp4_on("fp4_product_carried", "gain", gain, device)
+        resid = (r.data_ptr(), float(scale[0]) if scale else 1.0, gain.data_ptr(), dtype_code(gain.dtype), xg.data_ptr(), squares.data_ptr())
+    else:
+        dtype = out.dtype
+        if dtype is not torch.bfloat16 and (gated or dtype is not torch.float32):
+            raise TypeError(f"fp4_product_carried: results in {dtype}")
+        ldo = _fp4_rows("fp4_product_carried", "out", out, rows, N // 2 if gated else N, dtype, device)
+    if rows == 0:
+        return
+    _lib.check(_lib.load().he_fp4_product_carried(
+        _ptr(out), ldo, x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), rows, N, K, w.group, dtype_code(dtype),
+        F32 if bias is None else dtype_code(bias.dtype), gated, *_act4(act), owed, count, float(eps), *resid, _stream()))
+
+
 def fp4_experts_workspace_bytes(rows: int, top: int, gate_up, down) -> int:
     """Bytes of scratch memory that fp4_experts wants for so many rows of `top` choices."""
     E, D, I = down.shape

@@ -209,11 +209,36 @@ class Linear:
         return out
 
     def _run_fp4(self, x, rows, ctx, bias, out_dtype, out, sink):
-        x, out = self._dense(x, rows, ctx, out_dtype, out)
+        N = self.weight.shape[0]
+        if sink is not None and out is None and out_dtype == BF16 and self._carries(rows) and N % 4 == 0 \
+                and sink.stream.rows == rows and sink.stream.resid.shape[-1] == N:
+            gain, eps, *dyt = sink.norm.carried()
+            if not dyt:
+                xg, squares = ctx.alloc((rows, N), BF16), ctx.alloc((rows, -(-N // 16)), F32)
+                self._fp4(None, x, bias, rows, ctx, residual=(sink.stream.resid, gain, xg, squares, sink.scale))
+                sink.stream.prepared = (sink.norm, NormedRows(xg, squares, eps, rows))
+                return None
+        if out is None:
+            out = ctx.alloc((rows, N), out_dtype)
         self._fp4(out, x, bias, rows, ctx)
         return out
 
-    def _fp4(self, out, x, bias, rows: int, ctx: StepContext, **epilogue) -> None:
+    def _carries(self, rows: int) -> bool:
+        """Whether a packed weight's product carries a norm: few rows, whose norm kernels (4.7 us each for 8 rows of 3584) would be a seventh of a layer."""
+        return 0 < rows <= ops.FP4_CARRIED_ROWS and self.weight.shape[1] >= 8 and not self.ordered
+
+    def _fp4(self, out, x, bias, rows: int, ctx: StepContext, residual=None, **epilogue) -> None:
+        if isinstance(x, PieceRows):
+            raise TypeError("Linear: piece-major rows for a product that does not read them (ask reads_pieces)")
+        row_scale = None
+        if isinstance(x, NormedRows):
+            if self._carries(rows) and not x.pieces and not x.finished:
+                x, row_scale = x.scaled, (x.partials, x.eps)
+            else:
+                x = x.tensor(ctx)
+        if residual is not None or row_scale is not None:
+            ops.fp4_product_carried(out, x, self.weight, bias, rows, row_scale=row_scale, residual=residual, **epilogue)
+            return
         size = ops.fp4_product_workspace_bytes(rows, self.weight, bool(epilogue),
                                               whole=x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and rows * x.stride(0) < 1 << 31)
         ops.fp4_product(out, x, self.weight, bias, rows, workspace=ctx.scratch.transient((size,), torch.uint8) if size else None, **epilogue)
@@ -397,7 +422,7 @@ class Linear:
         if isinstance(self.weight, fp4.Fp4Weight):
             if out_pieces:
                 raise ValueError("Linear.gated_silu: a packed weight's product writes row-major (ask gated_pieces)")
-            self._fp4(out, x.tensor(ctx) if isinstance(x, NormedRows) else a, None, rows, ctx, gated=True, act=consts)
+            self._fp4(out, x, None, rows, ctx, gated=True, act=consts)
             return
         if rows <= ops.BLOCKSPLIT_PIECES_MAX_M:
             ops.gemm_blocksplit(out, a, self.weight, None, rows, gated=True, row_scale=scale,

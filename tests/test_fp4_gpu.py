@@ -431,3 +431,72 @@ def test_refusals(api):
     ops.fp4_experts(moe, x, stack, downs, ids, shares, 0, workspace=ws)
     torch.cuda.synchronize()
     assert (out == 7).all() and (moe == 7).all()
+
+
+@pytest.mark.parametrize("M,N,K,group,dtype", [(1, 64, 128, 64, BF16), (3, 100, 72, 32, F32), (8, 896, 1003, 64, BF16), (16, 3584, 512, 128, BF16), (13, 20, 9, 32, F32)])
+def test_a_norm_carried_across_two_products(api, M, N, K, group, dtype):
+    """The first product's results in the residual rows, r * gain and the sums of squares beside them; the second product over those,
+    with a bias, gated and in 32 bits. Rows behind the last stay as they were."""
+    fp4, ops = api
+    x, w, b = rnd(80, M, K), fp4.pack(rnd(81, N, K, scale=0.1).cuda(), group), rnd(82, N)
+    w2, b2 = fp4.pack(rnd(83, 36, N, scale=0.1).cuda(), group), rnd(84, 36)
+    gain, start = rnd(85, N, dtype=dtype), rnd(86, M + 1, N, dtype=F32)
+    values, values2 = w.unpack(F32).cpu().double(), w2.unpack(F32).cpu().double()
+    resid = start.cuda()
+    xg, squares = torch.full((M + 1, N), 7.0, dtype=BF16, device="cuda"), torch.full((M + 1, -(-N // 16)), 7.0, device="cuda")
+    ops.fp4_product_carried(None, x.cuda(), w, b.cuda(), M, residual=(resid, gain.cuda(), xg, squares, 0.5))
+    want = start[:M].double() + 0.5 * (x.double() @ values.T + b.double())
+    size = P.sum_bound(x, values, group)
+    got = resid.cpu()
+    # the sum's bound, then the bias, the product with 0.5 (exact) and the addition, each within half a place of what it gives
+    assert ((got[:M].double() - want).abs() <= 0.5 * size + 2.0 ** -23 * (want.abs() + (x.double() @ values.T).abs() + b.double().abs())).all()
+    assert torch.equal(got[M], start[M]) and (xg[M] == 7).all() and (squares[M] == 7).all()
+    r = got[:M].double()
+    assert ((xg[:M].cpu().double() - r * gain.double()).abs() <= (2.0 ** -8 + 2.0 ** -23) * (r * gain.double()).abs()).all()
+    parts = torch.nn.functional.pad(r ** 2, (0, -N % 16)).view(M, -1, 16).sum(-1)
+    assert ((squares[:M].cpu().double() - parts).abs() <= 16 * 2.0 ** -24 * parts).all()
+    eps = 1e-5
+    a, scale = xg[:M].cpu().double(), 1 / (squares[:M].cpu().double().sum(-1, keepdim=True) / N + eps).sqrt()
+    z, size2 = (a @ values2.T) * scale, P.sum_bound(a, values2, group) * scale
+    # the scale: a sum of up to 224 squares, a division, a root and a reciprocal in 32 bits
+    size2 = size2 + 16 * 2.0 ** -23 * z.abs()
+    for kind in (F32, BF16):
+        out = torch.full((M + 1, 36), 7.0, dtype=kind, device="cuda")
+        ops.fp4_product_carried(out, xg, w2, b2.cuda(), M, row_scale=(squares, eps))
+        full = z + b2.double()
+        assert ((out[:M].cpu().double() - full).abs() - size2 - (HALF[kind] + 2.0 ** -23) * full.abs()).max() <= 2.0 ** -23 * b2.abs().max() and (out[M] == 7).all()
+    out = torch.empty((M, 18), dtype=BF16, device="cuda")
+    ops.fp4_product_carried(out, xg, w2, None, M, gated=True, row_scale=(squares, eps))
+    exact, g, u = P.act(z), z[:, 0::2].abs(), z[:, 1::2].abs()
+    slack = 1.13 * size2[:, 0::2] * (u + size2[:, 1::2]) + (g + size2[:, 0::2]) * size2[:, 1::2] + 2.0 ** -20 * g * u * (1 + g)      # (as in test_gated_product)
+    assert ((out.cpu().double() - exact).abs() <= slack + HALF[BF16] * (exact.abs() + slack) + 2.0 ** -120).all()
+    # nothing owed and nothing carried: the product
+    plain, same = torch.empty((M, 36), dtype=F32, device="cuda"), torch.empty((M, 36), dtype=F32, device="cuda")
+    ops.fp4_product(plain, xg, w2, b2.cuda(), M)
+    ops.fp4_product_carried(same, xg, w2, b2.cuda(), M)
+    assert torch.equal(plain, same)
+
+
+def test_refusals_of_the_carried_product(api):
+    fp4, ops = api
+    w = fp4.pack(rnd(70, 32, 64).cuda(), 32)
+    x, out = rnd(73, 20, 64).cuda(), torch.full((20, 32), 7.0, device="cuda")
+    xg, squares, gain = torch.empty((20, 32), dtype=BF16, device="cuda"), torch.empty((20, 2), device="cuda"), torch.ones(32, device="cuda")
+    for rows in (17, -1):
+        with pytest.raises(ValueError, match="it takes up to 16"):
+            ops.fp4_product_carried(out, x, w, None, rows)
+    with pytest.raises(ValueError, match="row_scale"):
+        ops.fp4_product_carried(out, x, w, None, 4, row_scale=(squares[:3].contiguous(), 1e-5))
+    with pytest.raises(TypeError, match="row_scale"):
+        ops.fp4_product_carried(out, x, w, None, 4, row_scale=(xg, 1e-5))
+    with pytest.raises(ValueError, match="no output"):
+        ops.fp4_product_carried(out, x, w, None, 4, residual=(out, gain, xg, squares))
+    with pytest.raises(ValueError, match="squares"):
+        ops.fp4_product_carried(None, x, w, None, 4, residual=(out, gain, xg, squares[:, :1].contiguous()))
+    with pytest.raises(ValueError, match="gain"):
+        ops.fp4_product_carried(None, x, w, None, 4, residual=(out, gain[:16], xg, squares))
+    with pytest.raises(ValueError, match="multiple of 4"):
+        ops.fp4_product_carried(None, x, fp4.pack(rnd(71, 30, 64).cuda(), 32), None, 4, residual=(out, gain, xg, squares))
+    ops.fp4_product_carried(out, x, w, None, 0)
+    torch.cuda.synchronize()
+    assert (out == 7).all()
