@@ -69,13 +69,25 @@ def test_refusals_of_the_product(L):
     assert "groups of 48" in call(group=48)
     assert "a weight of [0, 64]" in call(N=0)
     assert "16-byte aligned" in call(codes=AT + 8) and "16-byte aligned" in call(codes=None) and "16-byte aligned" in call(scales=AT + 2)
-    assert "rows of 64 at distances" in call(M=-1) and "rows of 64 at distances" in call(ldx=63) and "rows of 64 at distances" in call(ldo=31)
+    assert "rows of 64 at distances" in call(M=-1) and "rows of 64 at distances" in call(ldx=63) and "results of 32 at distances of 31" in call(ldo=31)
     assert "rows of 64 at distances" in call(M=(1 << 22) + 1)
     assert "dtype code 7" in call(out_dtype=7)
     assert "gated" in call(gated=1, out_dtype=0) and "gated" in call(gated=1, out_dtype=1, bias=AT) and "gated" in call(gated=1, out_dtype=1, N=33)
     need = L.he_fp4_product_workspace_bytes(3, 32, 5, 1)
     assert need > 0 and "a workspace of" in call(M=3, K=5) and "a workspace of" in call(M=3, K=5, workspace=AT, size=need - 1) \
         and "a workspace of" in call(M=3, K=5, workspace=AT + 8, size=need)
+
+
+def test_refusals_of_the_carried_product(L):
+    def call(out=AT, M=4, N=32, K=64, ldo=32, group=32, out_dtype=0, gated=0, bias=None, owed=None, count=2, resid=None, gain=AT, carried=AT, squares=AT):
+        return refusal(L, L.he_fp4_product_carried(out, ldo, AT, K, AT, AT, bias, M, N, K, group, out_dtype, 0, gated, 1.0, 0.0, 0.0, 0.0, owed, count, 1e-5,
+                                                   resid, 1.0, gain, 0, carried, squares, None))
+    assert "17 rows" in call(M=17) and "rows of 7" in call(K=7) and "groups of 16" in call(group=16)
+    assert "0 sums of squares" in call(owed=AT, count=0)
+    for wrong in (dict(N=30), dict(gated=1), dict(out=AT, resid=AT), dict(gain=None), dict(carried=None), dict(squares=None), dict(resid=AT + 8), dict(carried=AT + 4)):
+        assert "results for the residual rows" in call(**{"out": None, "resid": AT, **wrong})
+    assert "dtype code 0 at distances of 31" in call(ldo=31) and "dtype code 5" in call(out_dtype=5) and "dtype code 0" in call(out=None)
+    assert "gated" in call(gated=1, out_dtype=0, ldo=16)
 
 
 def test_refusals_of_the_experts(L):
