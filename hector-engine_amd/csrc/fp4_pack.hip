@@ -171,7 +171,7 @@ extern "C" int he_fp4_pack(void* codes, void* scales, const void* w, int64_t ldw
   const int tiles = (N + FP4_ROWS - 1) / FP4_ROWS, blocks = (K + FP4_K - 1) / FP4_K;
   const int64_t total = (int64_t)matrices * tiles * blocks;
   if (total == 0) return 0;
-  HE_REQUIRE(total < (4ll << 31), "he_fp4_pack: %lld tiles are too many", (long long)total);
+  HE_REQUIRE(total < (1ll << 26), "he_fp4_pack: %lld tiles are too many", (long long)total);
   const unsigned grid = (unsigned)((total + 3) / 4);
   const int item = dtype == HE_BF16 ? 2 : 4;
   const bool whole = ldw * item % 16 == 0 && (int64_t)K * item % 16 == 0 && ((uintptr_t)w & 15) == 0;
@@ -199,7 +199,7 @@ extern "C" int he_fp4_unpack(void* out, const void* codes, const void* scales, i
   const int tiles = (N + FP4_ROWS - 1) / FP4_ROWS, blocks = (K + FP4_K - 1) / FP4_K;
   const int64_t total = (int64_t)matrices * tiles * blocks;
   if (total == 0) return 0;
-  HE_REQUIRE(total < (4ll << 31), "he_fp4_unpack: %lld tiles are too many", (long long)total);
+  HE_REQUIRE(total < (1ll << 26), "he_fp4_unpack: %lld tiles are too many", (long long)total);
   const unsigned grid = (unsigned)((total + 3) / 4);
   const bool whole = K % 8 == 0 && ((uintptr_t)out & 15) == 0;
 #define UNPACK(T, G) unpack_kernel<T, G><<<grid, 256, 0, (hipStream_t)stream>>>((T*)out, (const uint8_t*)codes, (const uint16_t*)scales, N, K, tiles, blocks, total, whole)

@@ -206,7 +206,7 @@ template <int MT, int NT>
 int run_tall(const Fp4Case& c, int mtiles, int slices, float* parts, hipStream_t s) {
   const int ntiles = (c.w.tiles + 4 * NT - 1) / (4 * NT);
   const int64_t total = (int64_t)mtiles * ntiles * slices;
-  HE_REQUIRE(total < (1 << 28), "he_fp4_product: %lld tiles are too many for one launch", (long long)total);
+  HE_REQUIRE(total < (1 << 24), "he_fp4_product: %lld tiles are too many for one launch", (long long)total);
   const unsigned grid = (unsigned)((total + HE_XCDS - 1) / HE_XCDS * HE_XCDS);
   if (c.w.group == 128) fp4_tall_kernel<MT, NT, 1><<<grid, 256, 0, s>>>(c, mtiles, ntiles, slices, parts);
   else if (c.w.group == 64) fp4_tall_kernel<MT, NT, 2><<<grid, 256, 0, s>>>(c, mtiles, ntiles, slices, parts);

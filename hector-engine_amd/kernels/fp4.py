@@ -46,6 +46,7 @@ class Fp4Weight:
 
     def _hold(self, codes, scales, shape, group) -> None:
         self._codes, self._scales, self._shape, self._group, self._index = codes, scales, shape, group, codes.get_device()
+        self.pointers = codes.data_ptr(), scales.data_ptr()
 
     codes = property(lambda self: self._codes)
     scales = property(lambda self: self._scales)

@@ -302,8 +302,13 @@ def gemm_blocksplit_blocks(M: int, N: int, K: int) -> int:
     return int(_lib.load().he_gemm_blocksplit_blocks(M, N, K))
 
 
+_SILU, _SILU4 = (1.0, 0.0, 0.0), (1.0, 0.0, 0.0, 0.0)
+
+
 def _act4(act) -> tuple:
     """(alpha, limit, up_shift, cubic) of a gated activation's constants, the last one 0 where it is left out."""
+    if act is _SILU:
+        return _SILU4
     return tuple(float(a) for a in act) + (0.0,) * (4 - len(act))
 
 
@@ -1397,11 +1402,13 @@ def chosen_experts(out, h_scratch, x, gate_up, down, ids, weights, dense, rows: 
 
 def _fp4_weight(name: str, w, dims: int) -> int:
     """The current device, which a launch goes to and the weight has to be on (an Fp4Weight checks its own tensors when it is made)."""
+    device = torch._C._cuda_getDevice()
+    if type(w) is _fp4.Fp4Weight and w._index == device and len(w._shape) == dims:
+        return device
     if not isinstance(w, _fp4.Fp4Weight):
         raise TypeError(f"{name}: expected a packed weight (kernels.fp4.pack), got {type(w).__name__}")
     if len(w.shape) != dims:
         raise ValueError(f"{name}: expected a packed weight of {dims} dims, got {w.shape}")
-    device = torch._C._cuda_getDevice()
     if w.device_index != device:
         raise ValueError(f"{name}: a weight on cuda:{w.device_index}, the current device is cuda:{device}")
     return device
@@ -1414,10 +1421,12 @@ def _fp4_on(name: str, what: str, t, device: int) -> None:
 
 def _fp4_rows(name: str, what: str, t, rows: int, cols: int, dtype, device: int) -> int:
     """The distance of the rows of a tensor [rows or more, cols] whose elements of a row are neighbours."""
+    shape = t.shape
+    if shape == (rows, cols) and t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+        return cols
     _fp4_on(name, what, t, device)
     if t.dtype is not dtype:
         raise TypeError(f"{name}: {what} is {t.dtype}, expected {dtype}")
-    shape = t.shape
     if len(shape) != 2 or shape[1] != cols or shape[0] < rows:
         raise ValueError(f"{name}: {what}{tuple(shape)} is not [{rows}, {cols}]")
     apart, step = t.stride()
@@ -1449,7 +1458,7 @@ def fp4_pack(packed, w) -> None:
     ld = w.stride(-2) if N > 1 else K
     if (K > 1 and w.stride(-1) != 1) or ld < K or (lead and lead[0] > 1 and w.stride(0) != N * ld):
         raise ValueError(f"fp4_pack: w's rows must be contiguous and lie evenly, strides {w.stride()}")
-    _lib.check(_lib.load().he_fp4_pack(packed.codes.data_ptr(), packed.scales.data_ptr(), w.data_ptr(), ld, lead[0] if lead else 1, N, K,
+    _lib.check(_lib.load().he_fp4_pack(*packed.pointers, w.data_ptr(), ld, lead[0] if lead else 1, N, K,
                                        packed.group, dtype_code(w.dtype), _stream()))
 
 
@@ -1460,7 +1469,7 @@ def fp4_unpack(out, packed) -> None:
     _need(out, "fp4_unpack: out", shape=packed.shape)
     _fp4_on("fp4_unpack", "out", out, device)
     *lead, N, K = packed.shape
-    _lib.check(_lib.load().he_fp4_unpack(out.data_ptr(), packed.codes.data_ptr(), packed.scales.data_ptr(), lead[0] if lead else 1, N, K,
+    _lib.check(_lib.load().he_fp4_unpack(out.data_ptr(), *packed.pointers, lead[0] if lead else 1, N, K,
                                          packed.group, dtype_code(out.dtype), _stream()))
 
 
@@ -1471,13 +1480,13 @@ def fp4_product_workspace_bytes(rows: int, w, gated: bool = False, whole: bool =
 
 
 @_op("fp4_product")
-def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.0, 0.0), workspace=None) -> None:
+def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=_SILU, workspace=None) -> None:
     """out[rows, N] (bfloat16 or float32) = x[rows, K] (bfloat16) . W^T (+ bias [N]) with a packed weight (kernels.fp4), sums in 32 bits;
     or, gated, out[rows, N / 2] (bfloat16, no bias) = act(gate, up) for a weight that alternates gate and up rows, act =
     (alpha, limit, up_shift[, cubic]) the activation's constants as silu_mul takes them. The rows of x and out may lie apart.
     workspace: uint8, fp4_product_workspace_bytes(rows, w, gated) or more; calls that may run at the same time need one each."""
     device = _fp4_weight("fp4_product", w, 2)
-    N, K = w.shape
+    N, K = w._shape
     if rows < 0:
         raise ValueError(f"fp4_product: {rows} rows")
     if gated and (N % 2 or bias is not None):
@@ -1487,7 +1496,7 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.
     if dtype is not torch.bfloat16 and (gated or dtype is not torch.float32):
         raise TypeError(f"fp4_product: results in {dtype}")
     ldo = _fp4_rows("fp4_product", "out", out, rows, N // 2 if gated else N, dtype, device)
-    if bias is not None:
+    if bias is not None and (bias.shape != (N,) or bias.get_device() != device or not bias.is_contiguous()):
         _need(bias, "fp4_product: bias", shape=(N,))
         _fp4_on("fp4_product", "bias", bias, device)
     L = _lib.load()
@@ -1495,8 +1504,9 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=(1.0, 0.
     ws, size = _fp4_workspace("fp4_product", workspace, L.he_fp4_product_workspace_bytes(rows, N, K, whole), device)
     if rows == 0:
         return
-    _lib.check(L.he_fp4_product(out.data_ptr(), ldo, x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), rows, N, K, w.group,
-                                dtype_code(dtype), F32 if bias is None else dtype_code(bias.dtype), gated, *_act4(act), ws, size, _stream()))
+    _lib.check(L.he_fp4_product(out.data_ptr(), ldo, x.data_ptr(), ldx, *w.pointers, _ptr(bias), rows, N, K, w.group,
+                                dtype_code(dtype), F32 if bias is None else dtype_code(bias.dtype), gated, *_act4(act), ws, size,
+                                torch._C._cuda_getCurrentRawStream(device)))
 
 
 FP4_CARRIED_ROWS = 16
@@ -1546,7 +1556,7 @@ def fp4_product_carried(out, x, w, bias, rows: int, *, gated: bool = False, act=
     if rows == 0:
         return
     _lib.check(_lib.load().he_fp4_product_carried(
-        _ptr(out), ldo, x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), _ptr(bias), rows, N, K, w.group, dtype_code(dtype),
+        _ptr(out), ldo, x.data_ptr(), ldx, *w.pointers, _ptr(bias), rows, N, K, w.group, dtype_code(dtype),
         F32 if bias is None else dtype_code(bias.dtype), gated, *_act4(act), owed, count, float(eps), *resid, _stream()))
 
 
@@ -1584,8 +1594,8 @@ def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0
     ws, size = _fp4_workspace("fp4_experts", workspace, L.he_fp4_experts_workspace_bytes(rows, top, E, I, D), device)
     if rows == 0:
         return
-    _lib.check(L.he_fp4_experts(out.data_ptr(), x.data_ptr(), ldx, gate_up.codes.data_ptr(), gate_up.scales.data_ptr(), down.codes.data_ptr(),
-                                down.scales.data_ptr(), ids.data_ptr(), weights.data_ptr(), rows, top, E, I, D, gate_up.group, down.group,
+    _lib.check(L.he_fp4_experts(out.data_ptr(), x.data_ptr(), ldx, *gate_up.pointers, *down.pointers,
+                                ids.data_ptr(), weights.data_ptr(), rows, top, E, I, D, gate_up.group, down.group,
                                 identity, *_act4(act), ws, size, _stream()))
 
 

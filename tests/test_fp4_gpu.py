@@ -500,3 +500,37 @@ def test_refusals_of_the_carried_product(api):
     ops.fp4_product_carried(out, x, w, None, 0)
     torch.cuda.synchronize()
     assert (out == 7).all()
+
+
+def test_offsets_past_32_bits(api):
+    """Rows of x that span more than 4 GiB, results that do, codes that do: the same bits as at small distances."""
+    fp4, ops = api
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("60 GiB of free GPU memory")
+    M, K = 70000, 128
+    room = torch.empty((M, 32768), dtype=BF16, device="cuda")
+    room[:, :K] = rnd(90, M, K).cuda()
+    for N in (64, 2048):
+        w = fp4.pack(rnd(91, N, K, scale=0.1).cuda(), 64)
+        ws = workspace(ops.fp4_product_workspace_bytes(M, w))
+        want, got = (torch.empty((M, N), dtype=BF16, device="cuda") for _ in range(2))
+        ops.fp4_product(want, room[:, :K].contiguous(), w, None, M, workspace=ws)
+        ops.fp4_product(got, room[:, :K], w, None, M, workspace=ws)
+        assert torch.equal(got, want)
+    x = room[:, :K].contiguous()
+    ops.fp4_product(room[:, 16384:16384 + 2048], x, w, None, M, workspace=ws)
+    assert torch.equal(room[:, 16384:16384 + 2048], want)
+    del room, want, got
+    # weight rows that repeat every 64: so do the results
+    few = rnd(92, 64, 65536, scale=0.02).cuda()
+    w = fp4.pack(few.repeat(2049, 1), 128)
+    assert w.codes.nbytes > 1 << 32
+    for M in (1, 16, 80):
+        x = rnd(93, M, 65536).cuda()
+        ws = workspace(ops.fp4_product_workspace_bytes(M, w))
+        out = torch.empty((M, w.shape[0]), dtype=F32, device="cuda")
+        ops.fp4_product(out, x, w, None, M, workspace=ws)
+        exact = x.double() @ fp4.pack(few, 128).unpack(F32).double().T
+        assert ((out[:, :64].double() - exact).abs().cpu() <= P.sum_bound(x, fp4.pack(few, 128).unpack(F32), 128)).all()
+        assert torch.equal(out.view(M, 2049, 64), out[:, None, :64].expand(M, 2049, 64))
+    torch.cuda.empty_cache()
