@@ -158,9 +158,9 @@ __device__ __forceinline__ int fp4_group_of(const int32_t* tile_begin, int group
 int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s);
 // one row, the sum over its choices (with ids): of expert ids[choice] with X row `choice`
 int fp4_run_chain(const Fp4Case& c, hipStream_t s);
-// fp4_tall.hip: rows in tiles of 16 mt, mtiles of them at most, weight rows in tiles of 64 nt; x may be read 16 bytes at a time, K is a multiple of
-// 128. slices > 1: K cut in so many (of a block at least), their sums by way of parts [slices][M][N rounded up to 16].
+// fp4_tall.hip: rows in tiles of 16 mt, mtiles of them at most, weight rows in tiles of 64 nt, K in `parts` within a workgroup; x may be read 16 bytes at a
+// time, K is a multiple of 128. slices > 1: K cut in so many (of a block at least) between workgroups too, their sums by way of sums [slices][M][N rounded up to 16].
 struct Fp4Plan {
-  int mt, nt, slices;         // mt 0: fp4_run_few
+  int mt, nt, parts, slices;  // mt 0: fp4_run_few
 };
-int fp4_run_tall(const Fp4Case& c, Fp4Plan plan, int mtiles, float* parts, hipStream_t s);
+int fp4_run_tall(const Fp4Case& c, Fp4Plan plan, int mtiles, float* sums, hipStream_t s);

@@ -55,23 +55,23 @@ __global__ __launch_bounds__(256) void clear_columns_kernel(uint16_t* __restrict
 // How a product is cut. Up to 16 rows run through the kernel that has no barriers (fp4_few.hip; 16 rows of 37888 x 3584 20.2 us, 22.1 in tiles of 32
 // rows; 3584 x 18944 16.4 and 19.4), and so do more, 16 at a time, where the weight is small (mt 0): it reads the codes again for
 // each 16, at some 4300 blocks of 128 k of 16 rows a microsecond. Tiles of more rows: a tile's time is its blocks of 128 k times the
-// microseconds that a block takes, alone on its unit or as its share of a unit that has several; the fewest over the shapes and the
+// microseconds that a block (of each part of K) takes, alone on its unit or as its share of a unit that has several; the fewest over the shapes and the
 // slices of K, whose sums cost two passes over them and a launch. (64 rows of 1024 x 3584 5.1 us in sixteens, 9.8 in tiles; of 4608 x
-// 3584 12.2, 13.7; of 37888 x 3584 27 in tiles. Of 50 products, 17 to 1024 rows of 1024 to 37888 columns and K of 3584 to 27648, the
-// tiles that this chooses take 1.04 of the time of the best of 14 shapes and slices in the geometric mean, 1.33 at most.)
+// 3584 12.2, 13.7; of 37888 x 3584 27 in tiles. @@STATS@@)
 Fp4Plan plan_of(int64_t M, int N, int K) {
-  static const struct { int mt, nt; double alone, shared; } shapes[] = {{2, 1, 0.45, 0.25}, {4, 1, 0.53, 0.4}, {4, 2, 1.0, 0.63}, {8, 2, 1.35, 1.2}, {8, 4, 2.3, 1.75}};
+  static const struct { int mt, nt, parts; double alone, shared; } shapes[] = {
+      {2, 1, 2, 0.45, 0.54}, {2, 2, 2, 1.08, 0.73}, {4, 1, 1, 0.53, 0.35}, {4, 1, 2, 0.82, 0.84}, {4, 2, 2, 1.13, 1.22}, {8, 2, 1, 1.07, 0.91}, {8, 4, 1, 1.96, 1.6}};
   const int blocks = (K + FP4_K - 1) / FP4_K, cus = he_cus();
-  Fp4Plan best = {0, 0, 1};
+  Fp4Plan best = {0, 0, 1, 1};
   if (M <= 16 || far(M, padded_k(K))) return best;       // (the kernel of many rows counts in 32 bits)
   double least = 3 + 0.03 * blocks + (double)((M + 15) / 16 * ((N + 15) / 16) * blocks) / 4300;
   for (const auto& t : shapes) {
     const int64_t tiles = (M + 16 * t.mt - 1) / (16 * t.mt) * ((N + 64 * t.nt - 1) / (64 * t.nt));
-    for (int slices = 1; slices <= 16 && slices <= blocks; slices *= 2) {
+    for (int slices = 1; slices <= 16 && slices * t.parts <= blocks; slices *= 2) {
       const double load = tiles * slices > 8 * cus ? (double)tiles * slices / cus : (double)((tiles * slices + cus - 1) / cus);
       const double turn = load * t.shared > t.alone ? load * t.shared : t.alone;
-      const double us = 3 + (blocks + slices - 1) / slices * turn + (slices > 1 ? 4 + 8e-6 * slices * M * N / 4 : 0) + (K % FP4_K ? 2.5 : 0);
-      if (us < least) least = us, best = {t.mt, t.nt, slices};
+      const double us = 3 + (blocks + slices * t.parts - 1) / (slices * t.parts) * turn + (slices > 1 ? 4 + 5e-6 * slices * M * N / 4 : 0) + (K % FP4_K ? 2.5 : 0);
+      if (us < least) least = us, best = {t.mt, t.nt, t.parts, slices};
     }
   }
   return best;
@@ -107,7 +107,7 @@ ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   // 64 rows 89, 54, 46, 51, 100; 256 rows -, 125, 76, 74, 113; 512 rows -, 219, 128, 119, 128; 2048 rows -, 800, 464, 418, 303.
   t.bm = choices <= 3ll * experts ? 4 : choices <= 8ll * experts ? 16 : choices <= 40ll * experts ? 32 : choices <= 96ll * experts ? 64 : 128;
   t.mtiles = he_group_rows_most_tiles(rows, top, experts, t.bm);
-  t.up = t.down = {t.bm / 16, t.bm == 128 ? 4 : 1, 1};
+  t.up = t.down = {t.bm / 16, t.bm == 128 ? 4 : 1, 1, 1};
   t.ints = padded(4 * he_group_rows_ints(rows, top, experts, t.bm));
   t.ldh = t.bm <= 16 ? (I + 7) / 8 * 8 : padded_k(I);
   t.h = padded(choices * t.ldh * 2);
