@@ -22,7 +22,9 @@ enum { ROWS_ALONE, CHOICES, NORM };
 // r^2, the second multiplies its sums by the row's scale, whose parts are read, all at once, while its first codes are on their way.
 template <int NT, int W, int D, int XL, int GROUPS, int KIND>
 __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[W * (NT > 2 * XL ? NT : 2 * XL) * 1024];
+  constexpr int WORDS = NT * GROUPS * 8, EACH_S = (WORDS + 63) / 64;           // the scales of a block, two a word; of a lane
+  constexpr int PLACE = XL * 1024 + WORDS * 4, OWN = 2 * PLACE > NT * 1024 ? 2 * PLACE : NT * 1024;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[W * OWN];
   constexpr bool CHAIN = KIND == CHOICES, CARRIED = KIND == NORM;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
   constexpr int ROWS = 4 * XL;                             // of a tile of rows
@@ -65,10 +67,16 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     else if (!CHAIN) x[i] += (c.rows_of ? (int64_t)max(c.rows_of[slot], 0) : min(slot, c.M - 1)) * c.ldx;
   }
   const int K = c.w.K;
-  uint8_t* own = lds + wave * (2 * XL * 1024);
+  uint8_t* own = lds + wave * OWN;
+  const uint32_t* scales[EACH_S];
+#pragma unroll
+  for (int i = 0; i < EACH_S; ++i) {
+    const int word = min(lane + 64 * i, WORDS - 1);
+    scales[i] = (const uint32_t*)c.w.scales + ((int64_t)group * c.w.tiles + min(tile0 + word / (8 * GROUPS), c.w.tiles - 1)) * blocks * (8 * GROUPS) + word % (8 * GROUPS);
+  }
 
   uint4 q[D][NT], xs[D][XL];
-  uint2 s[D][NT][GROUPS];
+  uint32_t s[D][EACH_S];
   auto load = [&](int u, int unit) {
     int kb = unit;
     int64_t from = 0, xfrom = 0;
@@ -82,14 +90,14 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     for (int j = 0; j < NT; ++j) {
       const int64_t at = tile_at[j] + from + kb;
       q[u][j] = he_load16_once<uint4>(c.w.codes + at * FP4_TILE_BYTES + lane * 16);
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) s[u][j][g] = *reinterpret_cast<const uint2*>(c.w.scales + at * (16 * GROUPS) + 16 * g + 4 * kq);
     }
+#pragma unroll
+    for (int i = 0; i < EACH_S; ++i) s[u][i] = scales[i][(from + kb) * (8 * GROUPS)];
     const int k = kb * FP4_K + 8 * r16;
 #pragma unroll
     for (int i = 0; i < XL; ++i) xs[u][i] = reinterpret_cast<const Piece*>(x[i] + xfrom + min(k, K - 8))->v;
   };
-  // X of a block into one of two places
+  // X and the scales of a block into one of two places
   auto keep = [&](int u, int unit, int place) {
     const int kb = CHAIN ? unit % blocks : unit;
     const int over = kb * FP4_K + 8 * r16 + 8 - K;         // (a piece over the end of its row was loaded from the row's last eight values)
@@ -104,8 +112,11 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
         const uint64_t lo = bits < 64 ? a >> bits | b << (64 - bits) : bits < 128 ? b >> (bits - 64) : 0, hi = bits < 64 ? b >> bits : 0;
         v = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
       }
-      *reinterpret_cast<uint4*>(own + place * (XL * 1024) + row * 256 + (r16 ^ row) * 16) = v;
+      *reinterpret_cast<uint4*>(own + place * PLACE + row * 256 + (r16 ^ row) * 16) = v;
     }
+#pragma unroll
+    for (int i = 0; i < EACH_S; ++i)
+      if (lane + 64 * i < WORDS) *reinterpret_cast<uint32_t*>(own + place * PLACE + XL * 1024 + (lane + 64 * i) * 4) = s[u][i];
   };
   const int xrow = min(r16, 4 * XL - 1);
   fp4_f32x4 acc[NT];
@@ -116,24 +127,27 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     fp4_bf16x8 v[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      v[t] = *reinterpret_cast<const fp4_bf16x8*>(own + place * (XL * 1024) + xrow * 256 + ((4 * t + kq) ^ xrow) * 16);
+      v[t] = *reinterpret_cast<const fp4_bf16x8*>(own + place * PLACE + xrow * 256 + ((4 * t + kq) ^ xrow) * 16);
+    // (every tile's products first: a product's sums are there some 30 cycles behind it)
+    fp4_f32x4 sums[NT][GROUPS];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const uint32_t words[4] = {q[u][j].x, q[u][j].y, q[u][j].z, q[u][j].w};
-      fp4_f32x4 part = {0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int j = 0; j < NT; ++j) {
+        const uint32_t words[4] = {q[u][j].x, q[u][j].y, q[u][j].z, q[u][j].w};
         const fp4_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_operand(words[t]), v[t],
-                                                       t % (4 / GROUPS) == 0 ? zero : part, 0, 0, 0);
-        if ((t + 1) % (4 / GROUPS) == 0) {
-          const uint2 b = s[u][j][t / (4 / GROUPS)];
-          const float f[4] = {__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u)};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(f[e], part[e], acc[j][e]);
-        }
+        constexpr int STEPS = 4 / GROUPS;
+        sums[j][t / STEPS] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_operand(words[t]), v[t], t % STEPS == 0 ? zero : sums[j][t / STEPS], 0, 0, 0);
       }
-    }
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint2 b = *reinterpret_cast<const uint2*>(own + place * PLACE + XL * 1024 + (j * GROUPS + g) * 32 + 8 * kq);
+        const float f[4] = {__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(f[e], sums[j][g][e], acc[j][e]);
+      }
   };
   if (lo < hi) {
 #pragma unroll
@@ -183,7 +197,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < NT; ++j) *reinterpret_cast<fp4_f32x4*>(lds + (wave * NT + j) * 1024 + lane * 16) = acc[j];
+  for (int j = 0; j < NT; ++j) *reinterpret_cast<fp4_f32x4*>(own + j * 1024 + lane * 16) = acc[j];
   __syncthreads();
   const int slot = m0 + r16;
   int to = slot;
@@ -197,7 +211,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   const int n = (tile0 + wave) * FP4_ROWS + 4 * kq;
   fp4_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < W; ++k) v += *reinterpret_cast<const fp4_f32x4*>(lds + (k * NT + wave) * 1024 + lane * 16);
+  for (int k = 0; k < W; ++k) v += *reinterpret_cast<const fp4_f32x4*>(lds + k * OWN + wave * 1024 + lane * 16);
   if (CARRIED && c.owed && to >= 0) v *= scale_of[r16];
   if (CARRIED && c.resid) {
     // (read ahead of the products they cost every kernel that carries a norm more than they saved this one)
