@@ -245,9 +245,17 @@ int run_few(const Fp4Case& c, int mtiles, hipStream_t s) {
 
 template <int XL, int KIND>
 int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
-  // Microseconds of (tiles, wavefronts, blocks ahead) = (1, 8, 2), (1, 8, 4), (2, 4, 2), (2, 8, 2), (4, 4, 2), weights from memory:
-  // 1 row of 4608 x 3584 5.0, 5.4, 5.5, 4.8, 7.0; 3584 x 18944 10.5, 9.3, 17.4, 12.4, 23.8; 5120 x 27648 19.8, 20.2, 25.0, 17.6, 33.5; 8 rows of
-  // 37888 x 3584 21.2, 23.3, 17.3, 17.6, 18.4; 16 rows of 10240 x 5120 15.3, 20.0, 12.9, 14.0, 10.7, of 3584 x 18944 16.4, 17.1, 20.5, 20.0, 26.5.
+  // Microseconds of (tiles, wavefronts, blocks ahead), weights in groups of 128 from memory: many tiles are best with many workgroups that hold
+  // little, few with many wavefronts to a tile.
+  //                      (1, 8, 2)  (2, 4, 2)  (2, 8, 2)  (4, 4, 2)  (4, 4, 1)
+  // 16 rows, 37888 x 3584     29.6       21.4       21.8       19.9       19.7    (groups of 32: 30.7, 24.8, 30.1, 28.2, 24.8)
+  // 16 rows, 10240 x 5120     15.0       13.8       14.6       11.2       13.8
+  // 16 rows, 4608 x 3584       8.4        6.8        6.9        8.4       10.4
+  // 8 rows, 37888 x 3584      23.3       18.4       18.5       17.8       16.8
+  // 8 rows, 20480 x 5120      18.5       15.8       16.0          -       17.0
+  // 1 row, 37888 x 3584       19.1       14.7       15.8       16.5       15.5
+  // 1 row, 4608 x 3584         5.5        5.9        5.3        7.3        9.2
+  // 1 row, 3584 x 18944       10.5       18.2       12.1       23.5       32.8    ((1, 8, 4): 9.5)
   const int64_t tiles = (int64_t)c.w.tiles * mtiles;
   if (tiles <= 256) {
     if constexpr (XL == 1) {
@@ -255,8 +263,14 @@ int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
     }
     return run_few<1, 8, 2, XL, KIND>(c, mtiles, s);
   }
-  if (XL == 4 && tiles >= 640) return run_few<4, 4, 2, XL, KIND>(c, mtiles, s);
-  return tiles <= 512 && c.w.blocks >= 64 ? run_few<2, 8, 2, XL, KIND>(c, mtiles, s) : run_few<2, 4, 2, XL, KIND>(c, mtiles, s);
+  if constexpr (XL == 4) {
+    if (tiles >= 1280) return run_few<4, 4, 1, XL, KIND>(c, mtiles, s);
+    if (tiles >= 640) return run_few<4, 4, 2, XL, KIND>(c, mtiles, s);
+  }
+  if constexpr (XL == 2) {
+    if (tiles >= 1536) return run_few<4, 4, 1, XL, KIND>(c, mtiles, s);
+  }
+  return tiles <= 512 && c.w.blocks >= 16 ? run_few<2, 8, 2, XL, KIND>(c, mtiles, s) : run_few<2, 4, 2, XL, KIND>(c, mtiles, s);
 }
 
 }  // namespace

@@ -52,12 +52,13 @@ __global__ __launch_bounds__(256) void clear_columns_kernel(uint16_t* __restrict
   if (at < rows * (ld - I)) h[at / (ld - I) * ld + I + at % (ld - I)] = 0;
 }
 
-// How a product is cut. Up to 16 rows run through the kernel that has no barriers (fp4_few.hip; 16 rows of 37888 x 3584 20.2 us, 22.1 in tiles of 32
+// How a product is cut. Up to 16 rows run through the kernel that has no barriers (fp4_few.hip; 16 rows of 37888 x 3584 20.8 us, 22 in tiles of 32
 // rows; 3584 x 18944 16.4 and 19.4), and so do more, 16 at a time, where the weight is small (mt 0): it reads the codes again for
 // each 16, at some 4300 blocks of 128 k of 16 rows a microsecond. Tiles of more rows: a tile's time is its blocks of 128 k times the
 // microseconds that a block (of each part of K) takes, alone on its unit or as its share of a unit that has several; the fewest over the shapes and the
-// slices of K, whose sums cost two passes over them and a launch. (64 rows of 1024 x 3584 5.1 us in sixteens, 9.8 in tiles; of 4608 x
-// 3584 12.2, 13.7; of 37888 x 3584 27 in tiles. @@STATS@@)
+// slices of K, whose sums cost two passes over them and a launch. (64 rows of 1024 x 3584 5.7 us in sixteens, 9.8 in tiles; of 4608 x 3584 11.1, 14; of
+// 37888 x 3584 65 by the estimate, 27 to 31 in tiles. The figures are fitted to 46 products of 17 to 2048 rows, 800 to 39472 columns and K of 768 to 23040 in 40
+// shapes and slices: what is chosen takes 1.02 of the time of the best in the geometric mean, 1.15 at most.)
 Fp4Plan plan_of(int64_t M, int N, int K) {
   static const struct { int mt, nt, parts; double alone, shared; } shapes[] = {
       {2, 1, 2, 0.45, 0.54}, {2, 2, 2, 1.08, 0.73}, {4, 1, 1, 0.53, 0.35}, {4, 1, 2, 0.82, 0.84}, {4, 2, 2, 1.13, 1.22}, {8, 2, 1, 1.07, 0.91}, {8, 4, 1, 1.96, 1.6}};
@@ -102,10 +103,11 @@ struct ExpertsScratch {
 ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   ExpertsScratch t = {};
   const int64_t choices = (int64_t)rows * top;
-  // A tile of rows should hold an expert's rows, of which there are more with some experts than with others. Microseconds in tiles of 4, 16, 32, 64,
-  // 128 rows of 16 experts of 2048 over rows of 2048, 4 chosen: 4 rows 30, 35, 39; 8 rows 38, 43, 46; 16 rows 42, 42, 46; 32 rows 60, 44, 43, 51, 100;
-  // 64 rows 89, 54, 46, 51, 100; 256 rows -, 125, 76, 74, 113; 512 rows -, 219, 128, 119, 128; 2048 rows -, 800, 464, 418, 303.
-  t.bm = choices <= 3ll * experts ? 4 : choices <= 8ll * experts ? 16 : choices <= 40ll * experts ? 32 : choices <= 96ll * experts ? 64 : 128;
+  // A tile of rows should hold an expert's rows, of which there are more with some experts than with others. Microseconds in tiles of 4, 8, 16, 32, 64,
+  // 128 rows of 16 experts of 2048 over rows of 2048, 4 chosen: 8 rows 29, 29, 36, 40; 16 rows 33, 32, 36, 44; 32 rows 47, 39, 37, 42, 49; 48 rows 59, 44, 41,
+  // 46, 49; 64 rows 73, 51, 44, 45, 49; 128 rows 122, 74, 62, 50, 52; 256 rows -, -, -, 80, 72, 102; 512 rows 120, 104, 107; 1024 rows 226, 199, 160. (64 rows in
+  // groups of 32: 57 in tiles of 16, 45 of 32.)
+  t.bm = choices <= 3ll * experts ? 4 : choices <= 5ll * experts ? 8 : choices <= 12ll * experts ? 16 : choices <= 40ll * experts ? 32 : choices <= 96ll * experts ? 64 : 128;
   t.mtiles = he_group_rows_most_tiles(rows, top, experts, t.bm);
   t.up = t.down = {t.bm / 16, t.bm == 128 ? 4 : 1, 1, 1};
   t.ints = padded(4 * he_group_rows_ints(rows, top, experts, t.bm));
