@@ -105,11 +105,12 @@ ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   const int64_t choices = (int64_t)rows * top;
   // A tile of rows should hold an expert's rows, of which there are more with some experts than with others. Microseconds in tiles of 4, 8, 16, 32, 64,
   // 128 rows of 16 experts of 2048 over rows of 2048, 4 chosen: 8 rows 29, 29, 36, 40; 16 rows 33, 32, 36, 44; 32 rows 47, 39, 37, 42, 49; 48 rows 59, 44, 41,
-  // 46, 49; 64 rows 73, 51, 44, 45, 49; 128 rows 122, 74, 62, 50, 52; 256 rows -, -, -, 80, 72, 102; 512 rows 120, 104, 107; 1024 rows 226, 199, 160. (64 rows in
-  // groups of 32: 57 in tiles of 16, 45 of 32.)
-  t.bm = choices <= 3ll * experts ? 4 : choices <= 5ll * experts ? 8 : choices <= 12ll * experts ? 16 : choices <= 40ll * experts ? 32 : choices <= 96ll * experts ? 64 : 128;
+  // 46, 49; 64 rows 73, 51, 44, 45, 49; 128 rows 122, 74, 62, 50, 53; 256 rows -, -, -, 80, 68, 100; 512 rows -, -, -, 127, 94, 112; 768 rows 181, 132, 124; 1536 rows
+  // 346, 233, 208. (64 rows in groups of 32: 57 in tiles of 16, 45 of 32.) Tiles of 64 rows are 128 columns wide (512 rows 94 us, 64 columns 109, whose rows
+  // are read twice as often), of 32 rows 64 (64 experts of 768, 128 rows, 8 chosen: 57 us, 59 with 128).
+  t.bm = choices <= 3ll * experts ? 4 : choices <= 5ll * experts ? 8 : choices <= 12ll * experts ? 16 : choices <= 32ll * experts ? 32 : choices <= 160ll * experts ? 64 : 128;
   t.mtiles = he_group_rows_most_tiles(rows, top, experts, t.bm);
-  t.up = t.down = {t.bm / 16, t.bm == 128 ? 4 : 1, 1, 1};
+  t.up = t.down = {t.bm / 16, t.bm / 32, 1, 1};
   t.ints = padded(4 * he_group_rows_ints(rows, top, experts, t.bm));
   t.ldh = t.bm <= 16 ? (I + 7) / 8 * 8 : padded_k(I);
   t.h = padded(choices * t.ldh * 2);

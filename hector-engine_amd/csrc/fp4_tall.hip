@@ -242,6 +242,7 @@ int fp4_run_tall(const Fp4Case& c, Fp4Plan plan, int mtiles, float* sums, hipStr
     case 222: return run_tall<2, 2, 2>(c, mtiles, plan.slices, sums, s);
     case 411: return run_tall<4, 1, 1>(c, mtiles, plan.slices, sums, s);
     case 412: return run_tall<4, 1, 2>(c, mtiles, plan.slices, sums, s);
+    case 421: return run_tall<4, 2, 1>(c, mtiles, plan.slices, sums, s);
     case 422: return run_tall<4, 2, 2>(c, mtiles, plan.slices, sums, s);
     case 821: return run_tall<8, 2, 1>(c, mtiles, plan.slices, sums, s);
     case 841: return run_tall<8, 4, 1>(c, mtiles, plan.slices, sums, s);
