@@ -279,7 +279,8 @@ int run_rows(const Fp4Case& c, int mtiles, hipStream_t s) {
 
 int fp4_run_chain(const Fp4Case& c, hipStream_t s) {
   HE_REQUIRE(c.w.K >= 8 && c.ids && c.choices >= 1 && c.choices <= 64 && c.M == 1, "he_fp4_experts: %d choices of a row", c.choices);
-  return c.w.tiles <= 256 ? run_few<1, 8, 2, 1, CHOICES>(c, 1, s) : run_few<2, 8, 2, 1, CHOICES>(c, 1, s);
+  // (two tiles a workgroup: 4 experts of 2048 over rows of 2048 12.7 us with the first product, 11.8 so; 2 of 4096 over 6144 19.5, 20.3; over 8192 the same)
+  return run_few<1, 8, 2, 1, CHOICES>(c, 1, s);
 }
 
 int fp4_run_few(const Fp4Case& c, int bm, int mtiles, hipStream_t s) {
