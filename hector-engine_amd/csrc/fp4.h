@@ -19,6 +19,10 @@ typedef __bf16 fp4_bf16x2 __attribute__((ext_vector_type(2)));
 typedef float fp4_f32x4 __attribute__((ext_vector_type(4)));
 typedef float fp4_f32x2 __attribute__((ext_vector_type(2)));
 
+// What lanes of a wavefront have written into LDS is there for its other lanes behind this: no instruction (the unit keeps the order), but without it
+// the compiler may take a lane's older read of a place for the new one where that lane has not written in between.
+__device__ __forceinline__ void fp4_written() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // eight codes as an operand
 __device__ __forceinline__ fp4_bf16x8 fp4_operand(uint32_t codes) {
   const fp4_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 1);

@@ -54,6 +54,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     const int base = __builtin_amdgcn_readlane(rank, lead);
     if (lane < 16) choice_in[wave][lane] = -1;
     if (id == group && rank >= base && rank < base + ROWS) choice_in[wave][rank - base] = lane;
+    fp4_written();
   }
   const int m0 = blockIdx.y * ROWS, tile0 = blockIdx.x * NT;
   int64_t tile_at[NT];
@@ -186,6 +187,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
 #pragma unroll
       for (int u = 0; u < D; ++u) {
         keep(u, kb + u, u & 1);
+        fp4_written();
         multiply(u, kb + u, u & 1);
         load(u, min(kb + D + u, hi - 1));
       }
@@ -194,6 +196,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     for (int u = 0; u < D; ++u)
       if (kb + u < hi) {
         keep(u, kb + u, u & 1);
+        fp4_written();
         multiply(u, kb + u, u & 1);
       }
   }

@@ -72,6 +72,7 @@ __global__ __launch_bounds__(256) void pack_kernel(uint8_t* __restrict__ codes, 
     }
 #pragma unroll
     for (int i = 0; i < 16 / AT_ONCE; ++i) *reinterpret_cast<uint4*>(own + (i * AT_ONCE + lane / PIECES) * ROW + piece * 16) = p[i];
+    fp4_written();
 #pragma unroll
     for (int t = 0; t < 4; ++t) eight(v[t], reinterpret_cast<const T*>(own + r * ROW), 32 * t + 8 * kq, FP4_K, true);
   } else {

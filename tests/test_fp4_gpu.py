@@ -122,6 +122,26 @@ def test_product_of_large_weights(api, M, N, K, group):
             assert ((got.cpu().double() - full).abs() <= slack + HALF[BF16] * (full.abs() + slack) + 2.0 ** -120).all(), xs
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 3, 4, 6, 8, 13, 16])
+@pytest.mark.parametrize("N,K", [(40, 8200), (300, 18944), (4100, 8192), (4608, 2100), (8200, 1104), (10250, 640), (21000, 512), (25000, 392)])
+def test_few_rows_of_every_shape(api, N, K, M, group):
+    """The numbers of weight rows and k at which few rows are cut another way, one to sixteen rows; a second call gives the same bits."""
+    fp4, ops = api
+    gen = torch.Generator(device="cuda").manual_seed(95)
+    x, w = torch.randn((M, K), generator=gen, device="cuda").to(BF16), torch.randn((N, K), generator=gen, device="cuda") * 0.05
+    # scales that differ from group to group and row to row by powers of two: a wrong one is not lost among the others
+    w *= torch.exp2(torch.randint(-3, 4, (N, -(-K // 32)), generator=gen, device="cuda")).repeat_interleave(32, 1)[:, :K]
+    packed = fp4.pack(w, group)
+    values = packed.unpack(F32).double()
+    want = x.double() @ values.T
+    size = (group + -(-K // group) + 16) * 2.0 ** -23 * (x.double().abs() @ values.abs().T)      # (as sum_bound)
+    out, again = torch.empty((M, N), dtype=F32, device="cuda"), torch.empty((M, N), dtype=F32, device="cuda")
+    ops.fp4_product(out, x, packed, None, M)
+    ops.fp4_product(again, x, packed, None, M)
+    assert ((out.double() - want).abs() <= size + 2.0 ** -24 * want.abs()).all() and torch.equal(out, again)
+
+
 @pytest.mark.parametrize("K", [1, 5, 7, 8, 9, 15, 121, 127, 129, 135, 255, 257])
 @pytest.mark.parametrize("M", [1, 6, 16, 21])
 def test_product_of_rows_that_end_anywhere(api, M, K):
