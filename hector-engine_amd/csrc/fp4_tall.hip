@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256 * PARTS, PARTS == 1 ? 2 : 1) void fp4_tall_kern
   const int m0 = mt * BM, tile0 = (nt * 4 + wave) * NT, blocks = c.w.blocks;
   const int pieces = slices * PARTS, piece_no = slice * PARTS + part;
   const int lo = (int)((int64_t)blocks * piece_no / pieces), hi = (int)((int64_t)blocks * (piece_no + 1) / pieces);
-  const int turns = (blocks + pieces - 1) / pieces;        // of the longest part
+  const int end = PARTS == 1 ? hi : lo + (blocks + pieces - 1) / pieces;       // (every part keeps the barriers of the longest)
   const uint8_t* codes[NT];
   const uint16_t* scales[NT];
 #pragma unroll
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256 * PARTS, PARTS == 1 ? 2 : 1) void fp4_tall_kern
     share_of[tid] = c.factor ? c.factor[slot] : 1.f;
   }
   uint32_t at = 0;
-  for (int kb = lo; kb < lo + turns; ++kb) {
+  for (int kb = lo; kb < end; ++kb) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (PARTS > 1 && kb >= hi) continue;

@@ -94,7 +94,8 @@ def test_product(api, M, N, K, group):
 
 
 @pytest.mark.parametrize("M,N,K,group", [(100, 4616, 1160, 64), (520, 4625, 1032, 128), (1100, 2052, 1003, 32), (400, 8200, 392, 32), (70, 9001, 3600, 64),
-                                         (48, 12300, 904, 128), (1030, 130, 4100, 64)])
+                                         (48, 12300, 904, 128), (1030, 130, 4100, 64), (155, 3630, 10112, 64), (805, 2515, 7380, 64), (141, 839, 16535, 128),
+                                         (33, 2000, 6272, 32)])
 def test_product_of_large_weights(api, M, N, K, group):
     """Sizes that the kernel of many rows takes, whole or in slices of K, at columns and k that end inside tiles: bias, gated, rows that lie apart."""
     fp4, ops = api
