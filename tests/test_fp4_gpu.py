@@ -257,7 +257,10 @@ def experts_case(seed, rows, E, top, I, D, group, act, holes=True):
     (1, 5, 8, 136, 72, 32, (1.702, 7.0, 1.0)), (1, 4, 3, 20, 36, 64, (1.0, 0.0, 0.0)), (1, 3, 64, 24, 40, 32, (1.0, 0.0, 0.0)),
     (20, 16, 4, 72, 136, 32, (1.0, 0.0, 0.0)), (16, 2, 4, 40, 80, 64, (1.0, 0.0, 0.0)), (40, 64, 2, 16, 48, 32, (1.0, 0.0, 0.0)),
     (150, 7, 2, 20, 36, 32, (1.702, 7.0, 1.0)), (3, 200, 8, 8, 16, 32, (1.0, 0.0, 0.0)), (400, 3, 2, 144, 264, 128, (1.0, 0.0, 0.0)),
-    (1, 3, 2, 3, 5, 32, (1.0, 0.0, 0.0)), (4, 4, 2, 9, 3, 64, (1.0, 0.0, 0.0)), (60, 2, 2, 3, 13, 32, (1.0, 0.0, 0.0)), (2, 2, 2, 1, 1, 32, (1.0, 0.0, 0.0))])
+    (1, 3, 2, 3, 5, 32, (1.0, 0.0, 0.0)), (4, 4, 2, 9, 3, 64, (1.0, 0.0, 0.0)), (60, 2, 2, 3, 13, 32, (1.0, 0.0, 0.0)), (2, 2, 2, 1, 1, 32, (1.0, 0.0, 0.0)),
+    (3, 4, 2, 512, 640, 128, (1.0, 0.0, 0.0)), (7, 4, 2, 512, 1280, 32, (1.0, 0.0, 0.0)), (17, 4, 2, 520, 2304, 64, (1.702, 7.0, 1.0)),
+    (40, 4, 2, 512, 640, 32, (1.0, 0.0, 0.0)), (200, 4, 2, 648, 1000, 128, (1.0, 0.0, 0.0)), (600, 4, 2, 256, 900, 64, (1.0, 0.0, 0.0)),
+    (1, 4, 4, 8200, 640, 128, (1.0, 0.0, 0.0)), (4, 4, 4, 8200, 320, 64, (1.0, 0.0, 0.0)), (1, 3, 2, 1032, 8200, 128, (1.0, 0.0, 0.0))])
 def test_experts(api, rows, E, top, I, D, group, act):
     fp4, ops = api
     gu, dn, x, ids, shares, exact, slack = experts_case(20, rows, E, top, I, D, group, act)
@@ -555,3 +558,30 @@ def test_offsets_past_32_bits(api):
         assert ((out[:, :64].double() - exact).abs().cpu() <= P.sum_bound(x, fp4.pack(few, 128).unpack(F32), 128)).all()
         assert torch.equal(out.view(M, 2049, 64), out[:, None, :64].expand(M, 2049, 64))
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M", [1, 7, 16])
+@pytest.mark.parametrize("N,K,group", [(40, 8200, 128), (300, 18944, 64), (4608, 2100, 32), (8200, 1104, 64), (10256, 640, 128), (25000, 392, 32)])
+def test_a_carried_norm_at_every_shape(api, N, K, group, M):
+    """The scale on the sums and the results in the residual rows, against the product without either: the same sums, so off by the roundings of
+    the scale (a sum of a few hundred squares, a division, a root, a reciprocal), the product with it and the addition alone."""
+    fp4, ops = api
+    gen = torch.Generator(device="cuda").manual_seed(96)
+    x, w = torch.randn((M, K), generator=gen, device="cuda").to(BF16), fp4.pack(torch.randn((N, K), generator=gen, device="cuda") * 0.05, group)
+    plain = torch.empty((M, N), dtype=F32, device="cuda")
+    ops.fp4_product(plain, x, w, None, M)
+    for count in (1, 65, 224, 700):
+        owed = torch.rand((M, count), generator=gen, device="cuda") * 3 * K / count
+        scale = 1 / (owed.double().sum(-1, keepdim=True) / K + 1e-5).sqrt()
+        out = torch.empty_like(plain)
+        ops.fp4_product_carried(out, x, w, None, M, row_scale=(owed, 1e-5))
+        want = plain.double() * scale
+        assert ((out.double() - want).abs() <= 2.0 ** -23 * (0.5 * (count / 64 + 12) + 4) * want.abs()).all()
+    start, gain = torch.randn((M, N), generator=gen, device="cuda"), torch.randn(N, generator=gen, device="cuda").to(BF16)
+    resid, xg, squares = start.clone(), torch.empty((M, N), dtype=BF16, device="cuda"), torch.empty((M, -(-N // 16)), device="cuda")
+    ops.fp4_product_carried(None, x, w, None, M, residual=(resid, gain, xg, squares))
+    want = start.double() + plain.double()
+    assert ((resid.double() - want).abs() <= 2.0 ** -23 * want.abs()).all()
+    assert ((xg.double() - resid.double() * gain.double()).abs() <= (2.0 ** -8 + 2.0 ** -23) * (resid.double() * gain.double()).abs()).all()
+    parts = torch.nn.functional.pad(resid.double() ** 2, (0, -N % 16)).view(M, -1, 16).sum(-1)
+    assert ((squares.double() - parts).abs() <= 16 * 2.0 ** -24 * parts).all()
