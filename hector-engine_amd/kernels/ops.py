@@ -1500,8 +1500,14 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=_SILU, w
         _need(bias, "fp4_product: bias", shape=(N,))
         _fp4_on("fp4_product", "bias", bias, device)
     L = _lib.load()
-    whole = ldx % 8 == 0 and x.data_ptr() % 16 == 0 and rows * ldx < 1 << 31
-    ws, size = _fp4_workspace("fp4_product", workspace, L.he_fp4_product_workspace_bytes(rows, N, K, whole), device)
+    if workspace is None:                # (one that is there is measured by the library)
+        whole = ldx % 8 == 0 and x.data_ptr() % 16 == 0 and rows * ldx < 1 << 31
+        ws, size = _fp4_workspace("fp4_product", None, L.he_fp4_product_workspace_bytes(rows, N, K, whole), device)
+    else:
+        if workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
+            _need(workspace, "fp4_product: workspace", torch.uint8)
+            _fp4_on("fp4_product", "workspace", workspace, device)
+        ws, size = workspace.data_ptr(), workspace.numel()
     if rows == 0:
         return
     _lib.check(L.he_fp4_product(out.data_ptr(), ldo, x.data_ptr(), ldx, *w.pointers, _ptr(bias), rows, N, K, w.group,

@@ -438,6 +438,16 @@ def test_refusals(api):
         ops.fp4_product(out[:, :16].to(BF16), x, w, torch.zeros(32, device="cuda"), 4, gated=True)
     with pytest.raises(TypeError, match="results in torch.float32"):
         ops.fp4_product(out[:, :16], x, w, None, 4, gated=True)
+    from hector_engine_amd.kernels.lib import KernelLibraryError
+    tall, wide, many = fp4.pack(rnd(74, 4096, 1160).cuda(), 32), rnd(75, 300, 1160).cuda(), torch.full((300, 4096), 7.0, device="cuda")
+    need = ops.fp4_product_workspace_bytes(300, tall)
+    assert need > 0
+    with pytest.raises(ValueError, match="a workspace of"):
+        ops.fp4_product(many, wide, tall, None, 300)
+    with pytest.raises(KernelLibraryError, match="a workspace of"):
+        ops.fp4_product(many, wide, tall, None, 300, workspace=workspace(ops.fp4_product_workspace_bytes(300, tall, whole=True) - 1))
+    with pytest.raises(TypeError, match="workspace"):
+        ops.fp4_product(many, wide, tall, None, 300, workspace=torch.empty(need, dtype=torch.int8, device="cuda"))
     ids, shares = torch.zeros((4, 2), dtype=torch.int32, device="cuda"), torch.zeros((4, 2), device="cuda")
     moe = torch.full((4, 64), 7.0, dtype=BF16, device="cuda")
     ws = workspace(ops.fp4_experts_workspace_bytes(4, 2, stack, downs))
@@ -454,7 +464,7 @@ def test_refusals(api):
     ops.fp4_product(out, x, w, None, 0)              # no rows: nothing happens
     ops.fp4_experts(moe, x, stack, downs, ids, shares, 0, workspace=ws)
     torch.cuda.synchronize()
-    assert (out == 7).all() and (moe == 7).all()
+    assert (out == 7).all() and (moe == 7).all() and (many == 7).all()
 
 
 @pytest.mark.parametrize("M,N,K,group,dtype", [(1, 64, 128, 64, BF16), (3, 100, 72, 32, F32), (8, 896, 1003, 64, BF16), (16, 3584, 512, 128, BF16), (13, 20, 9, 32, F32)])
