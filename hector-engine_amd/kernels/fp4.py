@@ -68,7 +68,7 @@ class Fp4Weight:
     def unpack(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, bfloat16 (exact) or float32."""
         from . import ops
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        out = self._codes.new_empty(self._shape, dtype=dtype)
         ops.fp4_unpack(out, self)
         return out
 
@@ -76,11 +76,11 @@ class Fp4Weight:
 def pack(w: torch.Tensor, group: int = 64) -> Fp4Weight:
     """Packs a float32 or bfloat16 matrix on the GPU (the rows of a matrix [N, K] may lie apart)."""
     from . import ops
-    shape, device = tuple(w.shape), w.device
+    shape = tuple(w.shape)
     codes, scales = storage_shapes(shape, group)
     if not w.is_cuda:
         raise ValueError("fp4.pack: expected a GPU tensor")
     packed = Fp4Weight.__new__(Fp4Weight)      # (its tensors are made here as its checks would have them)
-    packed._hold(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.bfloat16, device=device), shape, group)
+    packed._hold(w.new_empty(codes, dtype=torch.uint8), w.new_empty(scales, dtype=torch.bfloat16), shape, group)
     ops.fp4_pack(packed, w)
     return packed

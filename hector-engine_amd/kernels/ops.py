@@ -1451,12 +1451,14 @@ def _fp4_workspace(name: str, workspace, size: int, device: int):
 def fp4_pack(packed, w) -> None:
     """packed (kernels.fp4.Fp4Weight) = w, float32 or bfloat16, of its shape."""
     device = _fp4_weight("fp4_pack", packed, len(packed.shape))
-    _fp4_on("fp4_pack", "w", w, device)
-    if tuple(w.shape) != packed.shape:
+    if w.get_device() != device:
+        _fp4_on("fp4_pack", "w", w, device)
+    if w.shape != packed.shape:
         raise ValueError(f"fp4_pack: w{tuple(w.shape)} for a packed weight of {packed.shape}")
     *lead, N, K = packed.shape
-    ld = w.stride(-2) if N > 1 else K
-    if (K > 1 and w.stride(-1) != 1) or ld < K or (lead and lead[0] > 1 and w.stride(0) != N * ld):
+    together = w.is_contiguous()
+    ld = K if together or N == 1 else w.stride(-2)
+    if not together and ((K > 1 and w.stride(-1) != 1) or ld < K or (lead and lead[0] > 1 and w.stride(0) != N * ld)):
         raise ValueError(f"fp4_pack: w's rows must be contiguous and lie evenly, strides {w.stride()}")
     _lib.check(_lib.load().he_fp4_pack(*packed.pointers, w.data_ptr(), ld, lead[0] if lead else 1, N, K,
                                        packed.group, dtype_code(w.dtype), _stream()))
@@ -1466,8 +1468,9 @@ def fp4_pack(packed, w) -> None:
 def fp4_unpack(out, packed) -> None:
     """out (float32 or bfloat16, contiguous) = the values of a packed weight."""
     device = _fp4_weight("fp4_unpack", packed, len(packed.shape))
-    _need(out, "fp4_unpack: out", shape=packed.shape)
-    _fp4_on("fp4_unpack", "out", out, device)
+    if out.shape != packed.shape or out.get_device() != device or not out.is_contiguous():
+        _need(out, "fp4_unpack: out", shape=packed.shape)
+        _fp4_on("fp4_unpack", "out", out, device)
     *lead, N, K = packed.shape
     _lib.check(_lib.load().he_fp4_unpack(out.data_ptr(), *packed.pointers, lead[0] if lead else 1, N, K,
                                          packed.group, dtype_code(out.dtype), _stream()))
