@@ -37,8 +37,9 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   int group = 0;
   int id = -1;                                             // lane i: the expert of choice i, -1: none
   if (c.ids) {
-    if (lane < c.choices && c.shares[lane] != 0.f) id = c.ids[lane];
-    if (id >= c.groups) id = -1;
+    const int choice = min(lane, c.choices - 1), given = c.ids[choice];      // (both asked for at once)
+    const float share = c.shares[choice];
+    if (lane < c.choices && share != 0.f && given < c.groups) id = given;
   }
   if (c.tile_begin) {
     if ((int)blockIdx.y >= c.tile_begin[c.groups]) return;

@@ -239,8 +239,8 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
   hipStream_t s = (hipStream_t)stream;
   uint8_t* p = (uint8_t*)workspace;
   const int choices = rows * top;
-  // few choices are grouped by the products themselves: a launch less (1 row of 16 experts of 2048 over rows of 2048, 4 chosen, 18.9 us -> 15.0,
-  // its second product's sums taken over the choices too); by more than 16 every workgroup would search for longer than the launch takes
+  // few choices are grouped by the products themselves: a launch less (16 experts of 2048 over rows of 2048, 4 chosen: 1 row 16.2 us -> 11.5, its second
+  // product's sums taken over the choices too; 4 rows 24.9 -> 22.3); by many more every workgroup searches for longer than the launch takes (8 rows 28.0 -> 30.4)
   const bool by_ids = t.bm <= 16 && choices <= 16;
   GroupRows lists = {};
   int rc = 0;
