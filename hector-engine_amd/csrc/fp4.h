@@ -20,7 +20,8 @@ typedef float fp4_f32x4 __attribute__((ext_vector_type(4)));
 typedef float fp4_f32x2 __attribute__((ext_vector_type(2)));
 
 // What lanes of a wavefront have written into LDS is there for its other lanes behind this: no instruction (the unit keeps the order), but without it
-// the compiler may take a lane's older read of a place for the new one where that lane has not written in between.
+// the compiler may take a lane's older read of a place for the new one where that lane has not written in between. (And what has been read may be
+// written over behind it.)
 __device__ __forceinline__ void fp4_written() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // eight codes as an operand

@@ -190,6 +190,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
         keep(u, kb + u, u & 1);
         fp4_written();
         multiply(u, kb + u, u & 1);
+        fp4_written();
         load(u, min(kb + D + u, hi - 1));
       }
     }
@@ -199,6 +200,7 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
         keep(u, kb + u, u & 1);
         fp4_written();
         multiply(u, kb + u, u & 1);
+        fp4_written();
       }
   }
   __syncthreads();

@@ -168,9 +168,9 @@ __global__ __launch_bounds__(256 * PARTS, PARTS == 1 ? 2 : 1) void fp4_tall_kern
     for (int i = i0; i < i0 + FEW; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) *reinterpret_cast<fp4_f32x4*>(own + (16 * (i - i0) + r16) * ROW + (16 * j + 4 * kq) * 4) = acc[i][j];
-    // (one kind of results a loop: with the kinds told apart at each of them 128 x 256 results of K 2048 took 1.1 of the time)
     if (PARTS > 1) __syncthreads();
     else fp4_written();
+    // (one kind of results a loop: with the kinds told apart at each of them 128 x 256 results of K 2048 took 1.1 of the time)
     auto rows = [&](auto put) {
 #pragma unroll 4
       for (int r = lane / (4 * NT) + part * (16 * FEW / PARTS); r < (part + 1) * (16 * FEW / PARTS); r += 16 / NT) {
@@ -201,6 +201,7 @@ __global__ __launch_bounds__(256 * PARTS, PARTS == 1 ? 2 : 1) void fp4_tall_kern
         if (to_of[r] >= 0 && n < c.w.N) fp4_put<FP4_BF16>(c, v + bias, to_of[r], n, 1.f, whole);
       });
     }
+    fp4_written();
   }
 }
 
