@@ -120,16 +120,18 @@ ExpertsScratch experts_scratch(int rows, int top, int experts, int I, int D) {
   return t;
 }
 
-// out[row] = the sum over the row's choices, in their order, of those that an expert took (with a weight that is not zero), and of weight * x of those from `experts` on (x null:
-// they add nothing)
+// out[row] = plus[row] (or null) + the sum over the row's choices, in their order, of those that an expert took (with a weight that is not zero), and of weight * x of those from
+// `experts` on (x null: they add nothing)
 __global__ __launch_bounds__(256) void add_choices_kernel(uint16_t* __restrict__ out, const float* __restrict__ partial, const int32_t* __restrict__ ids,
-                                                          const float* __restrict__ weights, const uint16_t* __restrict__ x, int64_t ldx, int top,
-                                                          int experts, int D) {
+                                                          const float* __restrict__ weights, const uint16_t* __restrict__ x, int64_t ldx,
+                                                          const float* __restrict__ plus, int top, int experts, int D) {
   const int64_t row = blockIdx.y;
   const int d = 4 * (blockIdx.x * 256 + threadIdx.x);
   if (d >= D) return;
   const int n = min(4, D - d);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (plus)
+    for (int i = 0; i < n; ++i) sum[i] = plus[row * D + d + i];
   for (int k = 0; k < top; ++k) {
     const int64_t choice = row * top + k;
     const int id = ids[choice];
@@ -223,6 +225,13 @@ extern "C" int64_t he_fp4_experts_workspace_bytes(int rows, int top, int experts
 extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void* up_codes, const void* up_scales, const void* down_codes,
                               const void* down_scales, const void* ids_i32, const void* weights_f32, int rows, int top, int experts, int I, int D,
                               int group_up, int group_down, int identity, float alpha, float limit, float up_shift, float cubic, void* workspace, int64_t workspace_bytes, void* stream) {
+  return he_fp4_experts_plus(out, x, ldx, up_codes, up_scales, down_codes, down_scales, ids_i32, weights_f32, nullptr, rows, top, experts, I, D, group_up, group_down, identity,
+                             alpha, limit, up_shift, cubic, workspace, workspace_bytes, stream);
+}
+
+extern "C" int he_fp4_experts_plus(void* out, const void* x, int64_t ldx, const void* up_codes, const void* up_scales, const void* down_codes,
+                                   const void* down_scales, const void* ids_i32, const void* weights_f32, const void* plus_f32, int rows, int top, int experts, int I, int D,
+                                   int group_up, int group_down, int identity, float alpha, float limit, float up_shift, float cubic, void* workspace, int64_t workspace_bytes, void* stream) {
   HE_REQUIRE(rows >= 0 && top > 0 && experts > 0 && I > 0 && D > 0 && I <= (1 << 25), "he_fp4_experts: bad sizes");
   HE_REQUIRE(experts <= HE_GROUP_ROWS_MOST && rows <= 65535 && (int64_t)rows * top < (1 << 26), "he_fp4_experts: %d experts and %d rows are too many", experts, rows);
   HE_REQUIRE(ldx >= D, "he_fp4_experts: rows of %d at a distance of %lld", D, (long long)ldx);
@@ -268,6 +277,7 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
   }
   if (by_ids && rows == 1 && !identity) {
     down.M = 1, down.out = out, down.out_f32 = false;
+    down.bias = plus_f32, down.bias_dtype = HE_F32;        // (the one row of it)
     down.pairs = D % 4 == 0 && ((uintptr_t)out & 7) == 0;
     if ((rc = fp4_run_few(up, t.bm, t.mtiles, s))) return rc;
     return fp4_run_chain(down, s);
@@ -278,6 +288,6 @@ extern "C" int he_fp4_experts(void* out, const void* x, int64_t ldx, const void*
     if ((rc = fp4_run_tall(up, t.up, t.mtiles, nullptr, s)) || (rc = fp4_run_tall(down, t.down, t.mtiles, nullptr, s))) return rc;
   }
   add_choices_kernel<<<dim3((D + 1023) / 1024, rows), 256, 0, s>>>((uint16_t*)out, partial, (const int32_t*)ids_i32, (const float*)weights_f32,
-                                                                   identity ? (const uint16_t*)x : nullptr, ldx, top, experts, D);
+                                                                   identity ? (const uint16_t*)x : nullptr, ldx, (const float*)plus_f32, top, experts, D);
   return he_check_launch("he_fp4_experts");
 }

@@ -6,7 +6,7 @@
 #pragma once
 #include <stdint.h>
 
-#define HE_ABI_VERSION 32
+#define HE_ABI_VERSION 33
 
 #ifdef __cplusplus
 extern "C" {
@@ -477,6 +477,11 @@ int he_fp4_experts(void* out, const void* x, int64_t ldx, const void* up_codes, 
                    const void* down_scales, const void* ids_i32, const void* weights_f32, int rows, int top, int experts, int I, int D,
                    int group_up, int group_down, int identity, float alpha, float limit, float up_shift, float cubic, void* workspace,
                    int64_t workspace_bytes, void* stream);
+// The same with plus [rows][D] (float32, or null) added to the sums before they are rounded.
+int he_fp4_experts_plus(void* out, const void* x, int64_t ldx, const void* up_codes, const void* up_scales, const void* down_codes,
+                        const void* down_scales, const void* ids_i32, const void* weights_f32, const void* plus_f32, int rows, int top, int experts, int I,
+                        int D, int group_up, int group_down, int identity, float alpha, float limit, float up_shift, float cubic, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1576,11 +1576,12 @@ def fp4_experts_workspace_bytes(rows: int, top: int, gate_up, down) -> int:
 
 
 @_op("fp4_experts")
-def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0, 0.0), identity: bool = False, workspace=None) -> None:
+def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0, 0.0), identity: bool = False, plus=None, workspace=None) -> None:
     """A routed feed-forward over packed experts: out[rows, D] (bfloat16) = the sum over a row's choices c of weights[row, c] *
     down[e] act(gate[e] x, up[e] x) with e = ids[row, c]; an id that is no expert adds nothing, nor does a weight of 0; with identity an id from E on adds
     weights[row, c] * x. gate_up: packed [E, 2 I, D], gate i of an expert in row 2 i, its up in 2 i + 1; down: packed [E, D, I]; ids int32, weights float32
-    [rows, top]; x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. workspace: uint8,
+    [rows, top]; x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. plus: float32 [rows, D], added to the sums before they are
+    rounded (what a shared expert gives). workspace: uint8,
     fp4_experts_workspace_bytes(rows, top, gate_up, down) or more; calls that may run at the same time need one each."""
     device = _fp4_weight("fp4_experts", gate_up, 3)
     _fp4_weight("fp4_experts", down, 3)
@@ -1599,13 +1600,16 @@ def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0
     if ids.dim() != 2 or ids.shape[0] < rows or ids.shape[1] == 0 or weights.shape != ids.shape:
         raise ValueError(f"fp4_experts: ids{tuple(ids.shape)} and weights{tuple(weights.shape)} are not [{rows}, choices]")
     top = ids.shape[1]
+    if plus is not None:
+        _need(plus, "fp4_experts: plus", torch.float32)
+        _fp4_rows("fp4_experts", "plus", plus, rows, D, torch.float32, device)
     L = _lib.load()
     ws, size = _fp4_workspace("fp4_experts", workspace, L.he_fp4_experts_workspace_bytes(rows, top, E, I, D), device)
     if rows == 0:
         return
-    _lib.check(L.he_fp4_experts(out.data_ptr(), x.data_ptr(), ldx, *gate_up.pointers, *down.pointers,
-                                ids.data_ptr(), weights.data_ptr(), rows, top, E, I, D, gate_up.group, down.group,
-                                identity, *_act4(act), ws, size, _stream()))
+    _lib.check(L.he_fp4_experts_plus(out.data_ptr(), x.data_ptr(), ldx, *gate_up.pointers, *down.pointers,
+                                     ids.data_ptr(), weights.data_ptr(), _ptr(plus), rows, top, E, I, D, gate_up.group, down.group,
+                                     identity, *_act4(act), ws, size, _stream()))
 
 
 @_op("diff_heads")

@@ -28,7 +28,7 @@ uses, out += sigmoid(gate . n) * shared(n) (gate None: out += shared(n)), the do
 stored number an output to the logits. A shared expert without a gate whose activation is the experts' own joins their
 fused matrices as columns of weight 1: it costs no launch of its own.
 Packed (pack_weights): each expert's matrices in 4 bits, one operator for all of them and any number of rows (ops.fp4_experts); a shared
-expert's columns are then a feed-forward of their own beside it.
+expert's columns are then a feed-forward of their own, whose 32-bit results join the experts' sums.
 names: the suffixes of its tensors (router, router_bias, correction; expert e's are 'e<e>.' + gate / up / down).
 """
 from __future__ import annotations
@@ -175,21 +175,17 @@ class RoutedExperts(FeedForward):
         out = ctx.alloc((rows, self.hidden))
         for r0 in range(0, rows, _ROW_CHUNK):
             n = min(_ROW_CHUNK, rows - r0)
+            turn = ctx.scratch.mark()
+            common = None
+            if shared is not None:
+                h = ctx.alloc((n, self.shared_cols))
+                shared[0].gated_silu(x[r0:r0 + n], n, ctx, h, act={"alpha": self.alpha, "limit": self.limit, "up_shift": self.up_shift})
+                common = shared[1](h, n, ctx, out_dtype=torch.float32)
             size = ops.fp4_experts_workspace_bytes(n, self.top, up, down)
             ops.fp4_experts(out[r0:r0 + n], x[r0:r0 + n], up, down, ids[r0:r0 + n], weights[r0:r0 + n], n, act=act,
-                            identity=self.identity > 0, workspace=ctx.scratch.transient((size,), torch.uint8))
-        if shared is None:
-            return out
-        both = ctx.alloc((rows, self.hidden))
-        for r0 in range(0, rows, _ROW_CHUNK):
-            n = min(_ROW_CHUNK, rows - r0)
-            turn = ctx.scratch.mark()
-            h = ctx.alloc((n, self.shared_cols))
-            shared[0].gated_silu(x[r0:r0 + n], n, ctx, h, act={"alpha": self.alpha, "limit": self.limit, "up_shift": self.up_shift})
-            common = shared[1](h, n, ctx)
-            ops.scaled_sum(both[r0:r0 + n], out[r0:r0 + n], common, n, 1.0, 1.0)
+                            identity=self.identity > 0, plus=common, workspace=ctx.scratch.transient((size,), torch.uint8))
             ctx.scratch.release(turn)
-        return both
+        return out
 
     def _few_rows(self, rows: int, x, ctx: StepContext) -> bool:
         """Whether the step runs through the chosen experts alone (kernels.ops.chosen_experts): bfloat16 with the

@@ -1,0 +1,91 @@
+"""Parts over weights in 4 bits: what joins their sums, what is packed and what is kept."""
+import pytest
+import torch
+
+from tests.plain import fp4_plain as P
+from tests.test_fp4_gpu import experts_case, workspace
+from tests.test_tile_routes_gpu import context
+
+pytestmark = pytest.mark.gpu
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+def routed(E, I, S, D, **more):
+    """A routed feed-forward of one choice a row with a shared expert of S columns, packed, whose activations are bfloat16 numbers exactly: a gate is 96, where
+    silu(96) = 96 in 32 bits, an up six times one value of x. (part, tensors)."""
+    from hector_engine_amd.parts.base import BuildEnv, PartSpec, build_part
+    shared = {"feed_forward": PartSpec("gated_mlp", {"hidden_size": D, "intermediate_size": S}), "name": "shared"}
+    part = build_part("feed_forward", PartSpec("routed_experts", {
+        "hidden_size": D, "intermediate_size": I, "experts": E, "top": 1, "correction": False, "normalize": True, "shared": shared, **more}), "m.",
+        BuildEnv(torch.device("cuda:0"), BF16, True))
+    gen = torch.Generator().manual_seed(E + I)
+    t = {part._router: torch.randn((E, D), generator=gen).to(BF16)}
+    t[part._router][:, 0] = 0
+    for n, name in [(I, lambda k, e=e: part._name(e, k)) for e in range(E)] + [(S, lambda k: part.shared._names[k])]:
+        gate, up = torch.zeros((n, D)), torch.zeros((n, D))
+        gate[:, 0] = 6                                     # (a group's largest magnitude of 6 has the scale 1)
+        up[torch.arange(n), torch.randint(1, D, (n,), generator=gen)] = 6 * torch.where(torch.rand(n, generator=gen) < 0.5, 1.0, -1.0)
+        t[name("gate")], t[name("up")], t[name("down")] = gate.to(BF16), up.to(BF16), (torch.randn((D, n), generator=gen) * 0.1).to(BF16)
+    part.bind({k: v.cuda() for k, v in t.items()})
+    part.pack_weights(32)
+    return part, t
+
+
+@pytest.mark.parametrize("rows", [1, 2, 16, 40, 300])
+def test_a_shared_expert_joins_the_experts_sums_in_32_bits(rows):
+    """Nothing is rounded to bfloat16 between the second products and the layer's result: the sums' own bounds and half a step of the result."""
+    E, I, S, D = 4, 96, 160, 200
+    part, t = routed(E, I, S, D)
+    assert part.shared_cols == S
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.exp2(torch.randint(-8, -4, (rows, D), generator=gen).float()) * torch.where(torch.rand((rows, D), generator=gen) < 0.5, 1.0, -1.5)
+    x[:, 0] = 16
+    x = x.to(BF16)
+    got = part.forward(x.cuda(), context(rows))[:rows].cpu().double()
+    choice = (x.double() @ t[part._router].double().T).argmax(-1)
+
+    def feed_forward(name, which):
+        h = (x[which].double() @ t[name("gate")].double().T) * (x[which].double() @ t[name("up")].double().T)
+        assert torch.equal(h.to(BF16).double(), h)
+        down = P.values(t[name("down")], 32)
+        return h @ down.T, P.sum_bound(h, down, 32)
+    want, bound = feed_forward(lambda k: part.shared._names[k], slice(None))
+    for e in range(E):
+        own = choice == e
+        if own.any():
+            y, b = feed_forward(lambda k: part._name(e, k), own)
+            want[own], bound[own] = want[own] + y, bound[own] + b
+    # (an addition or two of 32 bits are within the sums' bounds, which allow a whole last place of the sum of magnitudes for each of 40 and more)
+    assert ((got - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("rows,E,top,I,D,group,act", [
+    (1, 16, 4, 40, 64, 64, (1.0, 0.0, 0.0)), (1, 4, 3, 20, 35, 32, (1.0, 0.0, 0.0)), (5, 8, 3, 24, 72, 32, (1.702, 7.0, 1.0)),
+    (20, 3, 3, 136, 127, 128, (1.0, 0.0, 0.0)), (40, 64, 2, 16, 48, 32, (1.0, 0.0, 0.0)), (150, 7, 2, 20, 36, 32, (1.702, 7.0, 1.0)),
+    (400, 3, 2, 144, 264, 128, (1.0, 0.0, 0.0))])
+def test_experts_with_rows_to_add(rows, E, top, I, D, group, act):
+    from hector_engine_amd.kernels import fp4, ops
+    gu, dn, x, ids, shares, exact, slack = experts_case(20, rows, E, top, I, D, group, act)
+    up, down = fp4.pack(gu.cuda(), group), fp4.pack(dn.cuda(), group)
+    plus = torch.randn((rows + 1, D), generator=torch.Generator().manual_seed(3))
+    out = torch.full((rows + 1, D), float("nan"), dtype=BF16, device="cuda")
+    for identity in (False, True):
+        ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, act=act, identity=identity, plus=plus.cuda(),
+                        workspace=workspace(ops.fp4_experts_workspace_bytes(rows, top, up, down)))
+        got, want = out.cpu().double(), exact + plus[:rows].double()
+        own = torch.zeros((rows, 1), dtype=F64)
+        if identity:
+            own = (shares.double() * (ids >= E)).sum(-1, keepdim=True)
+            want = want + own * x.double()
+        # an addition is off by half a last place of the sum so far; those of the experts' parts are in their slack
+        slack1 = slack + (2 * top + 2) * 2.0 ** -24 * (plus[:rows].double().abs() + own * x.double().abs())
+        assert got[rows].isnan().all()
+        assert ((got[:rows] - want).abs() <= slack1 + 2.0 ** -8 * (want.abs() + slack1)).all()
+        if rows > 1 and not identity:
+            assert torch.equal(got[rows - 1], plus[rows - 1].to(BF16).double())      # (a row of no expert)
+    with pytest.raises(TypeError, match="plus: expected torch.float32"):
+        ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, plus=plus.cuda().to(BF16))
+    with pytest.raises(ValueError, match="plus"):
+        ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, plus=plus[:, :-1].contiguous().cuda())
+    with pytest.raises(ValueError, match="plus"):
+        ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, plus=plus)
