@@ -61,15 +61,16 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   int64_t tile_at[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) tile_at[j] = ((int64_t)group * c.w.tiles + min(tile0 + j, c.w.tiles - 1)) * blocks;
-  // a lane's pieces of X: row 4 i + (lane >> 4), eight k from 8 (lane & 15) on (rows behind the last repeat it: each row's results are its own)
+  auto row_at = [&](int r) {                               // (rows behind the last repeat it: each row's results are its own)
+    int64_t row = 0;
+    if (c.ids && !CHAIN) row = max(choice_in[wave][r], 0) / c.top;
+    else if (!CHAIN) row = c.rows_of ? max(c.rows_of[m0 + r], 0) : min(m0 + r, c.M - 1);
+    return c.x + row * c.ldx;
+  };
+  // a lane's pieces of X: row 4 i + (lane >> 4), eight k from 8 (lane & 15) on
   const uint16_t* x[XL];
 #pragma unroll
-  for (int i = 0; i < XL; ++i) {
-    const int slot = m0 + 4 * i + kq;
-    x[i] = c.x;
-    if (c.ids && !CHAIN) x[i] += (int64_t)(max(choice_in[wave][4 * i + kq], 0) / c.top) * c.ldx;
-    else if (!CHAIN) x[i] += (c.rows_of ? (int64_t)max(c.rows_of[slot], 0) : min(slot, c.M - 1)) * c.ldx;
-  }
+  for (int i = 0; i < XL; ++i) x[i] = row_at(4 * i + kq);
   const int K = c.w.K;
   uint8_t* own = lds + wave * OWN;
   const uint32_t* scales[EACH_S];
@@ -206,6 +207,43 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < NT; ++j) *reinterpret_cast<fp4_f32x4*>(own + j * 1024 + lane * 16) = acc[j];
+  // A group's sum of x * code can leave the range of 32 bits where its scaled one does not (128 values of x from 4.4e35 on): a wavefront that ends with infinities
+  // or NaN takes those sums once more with the scales in the operands, as the kernel of many rows has them. (One tile after the other, each value by itself: with the
+  // loads of the loop above the kernels held so many more registers that 16 rows of 37888 x 3584 in groups of 32 took 26.3 us, 22.4 without; so 63 products of 1 to
+  // 16 rows take 1.008 of the time without in the geometric mean.)
+  bool off = false;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) off |= !(fabsf(acc[j][e]) < INFINITY);
+  if (__any(off)) {
+    const uint16_t* row = row_at(xrow);
+#pragma unroll 1
+    for (int j = 0; j < NT; ++j) {
+      fp4_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int step = 4 * lo; step < 4 * hi; ++step) {     // of 32 k
+        const int unit = step >> 2, t = step & 3, choice = CHAIN ? unit / blocks : 0, kb = unit - choice * blocks;
+        const int expert = CHAIN ? __builtin_amdgcn_readlane(id, choice) : group;
+        if (expert < 0) continue;
+        const int64_t at = ((int64_t)expert * c.w.tiles + min(tile0 + j, c.w.tiles - 1)) * blocks + kb;
+        const uint32_t codes = *reinterpret_cast<const uint32_t*>(c.w.codes + at * FP4_TILE_BYTES + lane * 16 + 4 * t);
+        const uint32_t scale = c.w.scales[at * (16 * GROUPS) + t * GROUPS / 4 * 16 + r16];
+        const int k = kb * FP4_K + 32 * t + 8 * kq;
+        const uint16_t* p = row + choice * c.ldx + k;
+        uint32_t words[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k + e < K) words[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+        const fp4_bf16x8 v = __builtin_bit_cast(fp4_bf16x8, make_uint4(words[0], words[1], words[2], words[3]));
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_values(codes, __uint_as_float(scale << 16)), v, sum, 0, 0, 0);
+      }
+      fp4_f32x4 kept = *reinterpret_cast<const fp4_f32x4*>(own + j * 1024 + lane * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kept[e] = fabsf(kept[e]) < INFINITY ? kept[e] : sum[e];      // (a row without numbers changes no other row's bits)
+      *reinterpret_cast<fp4_f32x4*>(own + j * 1024 + lane * 16) = kept;
+    }
+  }
   __syncthreads();
   const int slot = m0 + r16;
   int to = slot;
