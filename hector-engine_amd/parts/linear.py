@@ -78,9 +78,14 @@ class Linear:
         self._chosen: dict[tuple, routes.Route] = {}     # (rows, activations, fast) -> route, for one version of the table
         self._chosen_version = -1
 
+    @property
+    def packed(self) -> bool:
+        """Whether the weight is in 4 bits."""
+        return isinstance(self.weight, fp4.Fp4Weight)
+
     def pack(self, group: int) -> None:
         """The weight in 4 bits from here on (kernels.fp4), where the part allows it; the stored one is let go."""
-        if self.packable and not isinstance(self.weight, fp4.Fp4Weight):
+        if self.packable and not self.packed:
             self.weight = fp4.pack(self.weight, group)
             self._plans.clear()
             self._chosen.clear()
@@ -419,7 +424,7 @@ class Linear:
         act_dtype, a, scale, pieces = _operand(x)
         if not self.gated_silu_rows(rows, ctx, act_dtype):
             raise ValueError("Linear.gated_silu: not for these rows (ask gated_silu_rows)")
-        if isinstance(self.weight, fp4.Fp4Weight):
+        if self.packed:
             if out_pieces:
                 raise ValueError("Linear.gated_silu: a packed weight's product writes row-major (ask gated_pieces)")
             self._fp4(out, x, None, rows, ctx, gated=True, act=consts)
@@ -453,7 +458,7 @@ class Linear:
         9728 x 896 at 768 rows 22.5 beside 24.9, at 1400 36.4 beside 36.8; 29824 x 704 at 149 rows 1.21). With fewer tiles units idle (1024 x 256 at
         1000 rows 12.7, 8.0)."""
         N, K = self.weight.shape
-        if isinstance(self.weight, fp4.Fp4Weight) or not (K <= 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0 and N % 8 == 0
+        if self.packed or not (K <= 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0 and N % 8 == 0
                 and ops.tiles_read(x, self.weight) and self.own_tiles(rows, ctx)) or library_tuning.enabled():
             return 0             # (a tuned choice of the library has not been measured against)
         if self._rounds(rows, 128) <= 1:
@@ -469,7 +474,7 @@ class Linear:
         beside 85, 100 rows 58 beside 71); with several rows of tiles and less of them real 0.77 to 1.24 (259 x 28672 x 4096 100 us, the two 82,
         541 x 37888 x 2048 106 and 98), with tiles for less than 0.8 of the rounds up to 1.48. Only where a part allows it (one_round_tiles): see _long."""
         N, K = self.weight.shape
-        if isinstance(self.weight, fp4.Fp4Weight) or not (self.one_round_tiles and K > 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0
+        if self.packed or not (self.one_round_tiles and K > 1024 and isinstance(x, torch.Tensor) and x.dtype == BF16 and x.is_contiguous() and K % 64 == 0
                 and N % 8 == 0 and self.weight.is_contiguous() and ops.tiles_read(x, self.weight) and self.own_tiles(rows, ctx)) \
                 or library_tuning.enabled():
             return None
@@ -495,7 +500,7 @@ class Linear:
 
     def gated_pieces(self, rows: int) -> bool:
         """Whether gated_silu can write its result piece-major at this many rows."""
-        if isinstance(self.weight, fp4.Fp4Weight):
+        if self.packed:
             return False
         return rows <= ops.BLOCKSPLIT_PIECES_MAX_M or self._plan(rows)[1] == 1
 

@@ -79,7 +79,7 @@ class GatedMLP(FeedForward):
 
     def _gate(self, h, x, rows: int, ctx: StepContext) -> None:
         """h[rows, inter] = act(gate x, up x) of many rows: one kernel where the product takes the activation along."""
-        if self.gate_up.gated_silu_rows(rows, ctx, x.scaled.dtype if isinstance(x, NormedRows) else x.dtype):
+        if self.gate_up.packed and self.gate_up.gated_silu_rows(rows, ctx, x.scaled.dtype if isinstance(x, NormedRows) else x.dtype):
             self.gate_up.gated_silu(x, rows, ctx, h, act=self.act)
             return
         if isinstance(x, NormedRows) and self.gate_up.own_tiles(rows, ctx, x.scaled.dtype):

@@ -4,7 +4,7 @@ import torch
 
 from tests.plain import fp4_plain as P
 from tests.test_fp4_gpu import experts_case, workspace
-from tests.test_tile_routes_gpu import context
+from tests.test_tile_routes_gpu import bound_part, context
 
 pytestmark = pytest.mark.gpu
 BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
@@ -89,3 +89,23 @@ def test_experts_with_rows_to_add(rows, E, top, I, D, group, act):
         ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, plus=plus[:, :-1].contiguous().cuda())
     with pytest.raises(ValueError, match="plus"):
         ops.fp4_experts(out, x.cuda(), up, down, ids.cuda(), shares.cuda(), rows, plus=plus)
+
+
+@pytest.mark.parametrize("tail", [1, 16, 64])
+@pytest.mark.parametrize("ordered", [False, True])
+def test_the_last_rows_of_a_long_step(tail, ordered):
+    """A feed-forward of more than 8192 rows runs them in turns. With stored weights a short last turn is the product and the activation, gate and up rounded between
+    them; packed, it is what those rows give by themselves."""
+    from hector_engine_amd.kernels import ops
+    D, I, rows = 256, 512, 8192 + tail
+    part = bound_part("gated_mlp", {"hidden_size": D, "intermediate_size": I}, D ** -0.5)
+    part.gate_up.ordered = ordered
+    x = torch.randn((rows, D), generator=torch.Generator(device="cuda").manual_seed(tail), device="cuda").to(BF16)
+    last, ctx = x[8192:], context(tail)
+    got = part.forward(x, context(rows))
+    both, h = part.gate_up(last, tail, ctx), torch.empty((tail, I), dtype=BF16, device="cuda")
+    ops.silu_mul(h, both, tail, True)
+    assert torch.equal(got[8192:rows], part.down(h, tail, ctx)[:tail])
+    for lin in (part.gate_up, part.down):
+        lin.pack(64)
+    assert torch.equal(part.forward(x, context(rows))[8192:rows], part.forward(last, context(tail))[:tail])
