@@ -52,6 +52,12 @@ __global__ __launch_bounds__(256) void clear_columns_kernel(uint16_t* __restrict
   if (at < rows * (ld - I)) h[at / (ld - I) * ld + I + at % (ld - I)] = 0;
 }
 
+// The rows of a turn of a product: the kernel of many rows counts the bytes of X in 32 bits.
+int turn_rows(int M, int K) {
+  const int64_t most = ((1ll << 32) - 1) / (2 * padded_k(K));
+  return M <= most ? M : (int)(most >= 128 ? most / 128 * 128 : most / 16 * 16);
+}
+
 // How a product is cut. Up to 16 rows run through the kernel that has no barriers (fp4_few.hip; 16 rows of 37888 x 3584 20.8 us, 22 in tiles of 32
 // rows; 3584 x 18944 16.4 and 19.4), and so do more, 16 at a time, where the weight is small (mt 0): it reads the codes again for
 // each 16, at some 4300 blocks of 128 k of 16 rows a microsecond. Tiles of more rows: a tile's time is its blocks of 128 k times the
@@ -64,8 +70,9 @@ Fp4Plan plan_of(int64_t M, int N, int K) {
       {2, 1, 2, 0.45, 0.54}, {2, 2, 2, 1.08, 0.73}, {4, 1, 1, 0.53, 0.35}, {4, 1, 2, 0.82, 0.84}, {4, 2, 2, 1.13, 1.22}, {8, 2, 1, 1.07, 0.91}, {8, 4, 1, 1.96, 1.6}};
   const int blocks = (K + FP4_K - 1) / FP4_K, cus = he_cus();
   Fp4Plan best = {0, 0, 1, 1};
-  if (M <= 16 || far(M, padded_k(K))) return best;       // (the kernel of many rows counts in 32 bits)
-  double least = 3 + 0.03 * blocks + (double)((M + 15) / 16 * ((N + 15) / 16) * blocks) / 4300;
+  if (M <= 16) return best;
+  const int64_t sixteens = (M + 15) / 16;
+  double least = sixteens > 65535 ? INFINITY : 3 + 0.03 * blocks + (double)(sixteens * ((N + 15) / 16) * blocks) / 4300;      // (of a launch 65535 at most)
   for (const auto& t : shapes) {
     const int64_t tiles = (M + 16 * t.mt - 1) / (16 * t.mt) * ((N + 64 * t.nt - 1) / (64 * t.nt));
     for (int slices = 1; slices <= 16 && slices * t.parts <= blocks; slices *= 2) {
@@ -78,7 +85,7 @@ Fp4Plan plan_of(int64_t M, int N, int K) {
   return best;
 }
 
-// The scratch of a product: the rows, where the kernel cannot read them as they are, then the slices' sums.
+// The scratch of a product's turn: the rows, where the kernel cannot read them as they are, then the slices' sums.
 struct ProductScratch {
   Fp4Plan plan;
   bool copy;
@@ -91,6 +98,11 @@ ProductScratch product_scratch(int M, int N, int K, bool whole) {
   t.rows = t.copy ? padded(M * padded_k(K) * 2) : 0;
   t.bytes = t.rows + (t.plan.slices > 1 ? (int64_t)t.plan.slices * M * ((N + 15) / 16 * 16) * 4 : 0);
   return t;
+}
+// of all turns
+int64_t product_bytes(int M, int N, int K, bool whole) {
+  const int turn = turn_rows(M, K);
+  return std::max(product_scratch(turn, N, K, whole).bytes, M % turn ? product_scratch(M % turn, N, K, whole).bytes : 0);
 }
 
 // The scratch of the experts of a step: the lists of he_group_rows, the activations and the results of each choice, and X where its
@@ -153,7 +165,7 @@ __global__ __launch_bounds__(256) void add_choices_kernel(uint16_t* __restrict__
 }  // namespace
 
 extern "C" int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int whole) {
-  return M <= 0 || N <= 0 || K <= 0 ? 0 : product_scratch(M, N, K, whole).bytes;
+  return M <= 0 || N <= 0 || K <= 0 ? 0 : product_bytes(M, N, K, whole);
 }
 
 // the case of he_fp4_product without its results
@@ -186,13 +198,24 @@ extern "C" int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx
   if (M == 0) return 0;
   results(&c, out, ldo, out_dtype, gated, {alpha, limit, up_shift, cubic});
   hipStream_t s = (hipStream_t)stream;
-  const ProductScratch t = product_scratch(M, N, K, c.whole && !far(M, ldx));
-  HE_REQUIRE(t.bytes == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= t.bytes),
-             "he_fp4_product: a workspace of %lld bytes, 16-byte aligned, is needed", (long long)t.bytes);
-  if (t.copy)
-    if (const int rc = pad_rows(&c, workspace, s)) return rc;
-  if (t.plan.mt == 0) return fp4_run_few(c, M > 8 ? 16 : M > 4 ? 8 : 4, (M + 15) / 16, s);
-  return fp4_run_tall(c, t.plan, (M + 16 * t.plan.mt - 1) / (16 * t.plan.mt), (float*)((uint8_t*)workspace + t.rows), s);
+  const int turn = turn_rows(M, K);
+  const bool whole = c.whole && !far(turn, ldx);
+  const ProductScratch first = product_scratch(turn, N, K, whole), last = M % turn ? product_scratch(M % turn, N, K, whole) : first;
+  const int64_t need = std::max(first.bytes, last.bytes);
+  HE_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need),
+             "he_fp4_product: a workspace of %lld bytes, 16-byte aligned, is needed", (long long)need);
+  for (int r0 = 0; r0 < M; r0 += turn) {
+    Fp4Case part = c;
+    const int n = part.M = std::min(turn, M - r0);
+    part.x += r0 * ldx, part.out = (uint8_t*)out + r0 * ldo * (c.out_f32 ? 4 : 2);
+    const ProductScratch& t = n == turn ? first : last;
+    if (t.copy)
+      if (const int rc = pad_rows(&part, workspace, s)) return rc;
+    const int rc = t.plan.mt == 0 ? fp4_run_few(part, n > 8 ? 16 : n > 4 ? 8 : 4, (n + 15) / 16, s)
+                                  : fp4_run_tall(part, t.plan, (n + 16 * t.plan.mt - 1) / (16 * t.plan.mt), (float*)((uint8_t*)workspace + t.rows), s);
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 extern "C" int he_fp4_product_carried(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M,

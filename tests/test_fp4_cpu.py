@@ -126,3 +126,22 @@ def test_the_route_of_packed_weights():
     from hector_engine_amd.kernels import routes
     import hector_engine_amd.parts.linear  # noqa: F401
     assert [r.name for r in routes.routes_of("linear", ("fp4", torch.bfloat16))] == ["fp4"]
+
+
+def test_rows_that_span_4_gib_run_in_turns(L):
+    """The kernel of many rows counts the bytes of its rows in 32 bits: a product of more runs in turns of whole tiles, which want one turn's workspace."""
+    def wants(M, N, K, whole=1):
+        return L.he_fp4_product_workspace_bytes(M, N, K, whole)
+    turn = ((1 << 32) - 1) // (2 * 1024) // 128 * 128
+    assert wants(turn, 2048, 1000) == wants(1 << 21, 2048, 1000) == wants(2 * turn, 2048, 1000) == wants(1 << 22, 2048, 1000) == turn * 1024 * 2
+    assert wants(1 << 22, 2048, 1024) == 0 and wants(1 << 22, 2048, 1024, 0) == turn * 1024 * 2
+    # a turn of a few rows of the largest K
+    assert wants(64, 16, 1 << 26) == wants(16, 16, 1 << 26) == 0
+
+
+def test_sixteen_rows_at_a_time_end_where_a_launch_does(L):
+    """Small weights run 16 rows at a time, of which a launch has 65535; more rows go to the kernel of many rows, which copies what is not whole blocks of 128."""
+    def wants(M, N, K, whole=1):
+        return L.he_fp4_product_workspace_bytes(M, N, K, whole)
+    assert wants(65535 * 16, 16, 100) == 0 and wants(65535 * 16 + 1, 16, 100) == (65535 * 16 + 1) * 128 * 2
+    assert wants(65535 * 16, 16, 7) == 65535 * 16 * 128 * 2 and wants(1 << 22, 16, 128) == 0
