@@ -54,8 +54,8 @@ __global__ __launch_bounds__(256) void clear_columns_kernel(uint16_t* __restrict
 
 // The rows of a turn of a product: the kernel of many rows counts the bytes of X in 32 bits.
 int turn_rows(int M, int K) {
-  const int64_t most = ((1ll << 32) - 1) / (2 * padded_k(K));
-  return M <= most ? M : (int)(most >= 128 ? most / 128 * 128 : most / 16 * 16);
+  const int64_t most = ((1ll << 32) - 1) / (2 * padded_k(K)), tile = most >= 128 ? 128 : 16;
+  return (int)std::min<int64_t>(M, most / tile * tile);
 }
 
 // How a product is cut. Up to 16 rows run through the kernel that has no barriers (fp4_few.hip; 16 rows of 37888 x 3584 20.8 us, 22 in tiles of 32
@@ -103,6 +103,25 @@ ProductScratch product_scratch(int M, int N, int K, bool whole) {
 int64_t product_bytes(int M, int N, int K, bool whole) {
   const int turn = turn_rows(M, K);
   return std::max(product_scratch(turn, N, K, whole).bytes, M % turn ? product_scratch(M % turn, N, K, whole).bytes : 0);
+}
+
+// Of any number of rows up to M: fewer rows may be cut into more slices (3584 x 18944: 512 rows in 4, 513 in none). Costs of slices grow evenly within sixteen rows, all
+// others stay: where the first and the last of them have one plan, so have those between. Where every shape has more than eight tiles a unit none has slices.
+int64_t most_product_bytes(int M, int N, int K, bool whole) {
+  M = turn_rows(M, K);
+  int64_t most = product_scratch(M, N, K, whole).bytes;
+  for (int lo = 17; lo <= M; lo += 16) {
+    if ((int64_t)(lo + 127) / 128 * ((N + 255) / 256) > 8 * he_cus()) {
+      for (int hi = M; (!whole || K % FP4_K) && hi >= lo; hi = (hi - 1) / 16 * 16)      // the rows alone, of the last that are copied
+        if (const ProductScratch t = product_scratch(hi, N, K, whole); t.plan.mt) return std::max(most, t.bytes);
+      return most;
+    }
+    const ProductScratch a = product_scratch(lo, N, K, whole), b = product_scratch(std::min(lo + 15, M), N, K, whole);
+    most = std::max({most, a.bytes, b.bytes});
+    if (a.plan.slices == b.plan.slices && !a.plan.mt == !b.plan.mt) continue;
+    for (int m = lo + 1; m < std::min(lo + 15, M); ++m) most = std::max(most, product_scratch(m, N, K, whole).bytes);
+  }
+  return most;
 }
 
 // The scratch of the experts of a step: the lists of he_group_rows, the activations and the results of each choice, and X where its
@@ -165,6 +184,9 @@ __global__ __launch_bounds__(256) void add_choices_kernel(uint16_t* __restrict__
 }  // namespace
 
 extern "C" int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int whole) {
+  return M <= 0 || N <= 0 || K <= 0 ? 0 : most_product_bytes(M, N, K, whole);
+}
+extern "C" int64_t he_fp4_product_call_bytes(int M, int N, int K, int whole) {
   return M <= 0 || N <= 0 || K <= 0 ? 0 : product_bytes(M, N, K, whole);
 }
 

@@ -457,8 +457,10 @@ int he_fp4_pack(void* codes, void* scales, const void* w, int64_t ldw, int matri
 int he_fp4_unpack(void* out, const void* codes, const void* scales, int matrices, int N, int K, int group, int dtype, void* stream);
 // out[M][N] (float32 or bfloat16, rows ldo apart) = x[M][K] (bfloat16, rows ldx apart) . W^T (+ bias); gated: bf16 [M][N / 2] of a weight
 // that alternates gate and up rows, the activation's constants as he_gated_act takes them. workspace: he_fp4_product_workspace_bytes
-// (whole: each row of x begins at a multiple of 16 bytes, and they span less than 4 GiB).
+// (whole: each row of x begins at a multiple of 16 bytes, and they span less than 4 GiB), which is enough for any fewer rows too; a call itself asks for
+// he_fp4_product_call_bytes, of which fewer rows may want more.
 int64_t he_fp4_product_workspace_bytes(int M, int N, int K, int whole);
+int64_t he_fp4_product_call_bytes(int M, int N, int K, int whole);
 int he_fp4_product(void* out, int64_t ldo, const void* x, int64_t ldx, const void* codes, const void* scales, const void* bias, int M, int N,
                    int K, int group, int out_dtype, int bias_dtype, int gated, float alpha, float limit, float up_shift, float cubic,
                    void* workspace, int64_t workspace_bytes, void* stream);

@@ -119,6 +119,7 @@ _SIGNATURES = {
     "he_fp4_pack": [c_ptr, c_ptr, c_ptr, c_i64, c_int, c_int, c_int, c_int, c_int, c_ptr],
     "he_fp4_unpack": [c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_ptr],
     "he_fp4_product_workspace_bytes": [c_int, c_int, c_int, c_int],
+    "he_fp4_product_call_bytes": [c_int, c_int, c_int, c_int],
     "he_fp4_product": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32,
                        c_f32, c_f32, c_ptr, c_i64, c_ptr],
     "he_fp4_product_carried": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_f32, c_f32,
@@ -170,6 +171,7 @@ _RESTYPES = {
     "he_gemm_plain_workspace_floats": c_i64,
     "he_routed_groups_ints": c_i64,
     "he_fp4_product_workspace_bytes": c_i64,
+    "he_fp4_product_call_bytes": c_i64,
     "he_fp4_experts_workspace_bytes": c_i64,
     "he_attention_decode_workspace_floats": c_i64,
     "he_attention_decode_fused_workspace_floats": c_i64,

@@ -1476,10 +1476,12 @@ def fp4_unpack(out, packed) -> None:
                                          packed.group, dtype_code(out.dtype), _stream()))
 
 
-def fp4_product_workspace_bytes(rows: int, w, gated: bool = False, whole: bool = False) -> int:
-    """Bytes of scratch memory that fp4_product wants for this weight and so many rows, gated or not (0: none). whole: each row of x begins at a
-    multiple of 16 bytes, and they span less than 4 GiB, so that none has to be copied for that."""
-    return int(_lib.load().he_fp4_product_workspace_bytes(rows, *w.shape, whole))
+def fp4_product_workspace_bytes(rows: int, w, gated: bool = False, whole: bool = False, alone: bool = False) -> int:
+    """Bytes of scratch memory that fp4_product wants for this weight and so many rows or any fewer, gated or not, which makes no difference (0: none). whole: each
+    row of x begins at a multiple of 16 bytes, and they span less than 4 GiB, so that none has to be copied for that. alone: for exactly this number of rows, of which
+    fewer may want more (a product of fewer rows is cut along K more often)."""
+    L = _lib.load()
+    return int((L.he_fp4_product_call_bytes if alone else L.he_fp4_product_workspace_bytes)(rows, *w.shape, whole))
 
 
 @_op("fp4_product")
@@ -1487,7 +1489,7 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=_SILU, w
     """out[rows, N] (bfloat16 or float32) = x[rows, K] (bfloat16) . W^T (+ bias [N]) with a packed weight (kernels.fp4), sums in 32 bits;
     or, gated, out[rows, N / 2] (bfloat16, no bias) = act(gate, up) for a weight that alternates gate and up rows, act =
     (alpha, limit, up_shift[, cubic]) the activation's constants as silu_mul takes them. The rows of x and out may lie apart.
-    workspace: uint8, fp4_product_workspace_bytes(rows, w, gated) or more; calls that may run at the same time need one each."""
+    workspace: uint8, fp4_product_workspace_bytes(rows, w) or more, which serves calls of fewer rows too; calls that may run at the same time need one each."""
     device = _fp4_weight("fp4_product", w, 2)
     N, K = w._shape
     if rows < 0:
@@ -1505,7 +1507,7 @@ def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=_SILU, w
     L = _lib.load()
     if workspace is None:                # (one that is there is measured by the library)
         whole = ldx % 8 == 0 and x.data_ptr() % 16 == 0 and rows * ldx < 1 << 31
-        ws, size = _fp4_workspace("fp4_product", None, L.he_fp4_product_workspace_bytes(rows, N, K, whole), device)
+        ws, size = _fp4_workspace("fp4_product", None, L.he_fp4_product_call_bytes(rows, N, K, whole), device)
     else:
         if workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
             _need(workspace, "fp4_product: workspace", torch.uint8)

@@ -244,7 +244,7 @@ class Linear:
         if residual is not None or row_scale is not None:
             ops.fp4_product_carried(out, x, self.weight, bias, rows, row_scale=row_scale, residual=residual, **epilogue)
             return
-        size = ops.fp4_product_workspace_bytes(rows, self.weight, bool(epilogue),
+        size = ops.fp4_product_workspace_bytes(rows, self.weight, alone=True,
                                               whole=x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and rows * x.stride(0) < 1 << 31)
         ops.fp4_product(out, x, self.weight, bias, rows, workspace=ctx.scratch.transient((size,), torch.uint8) if size else None, **epilogue)
 

@@ -145,3 +145,29 @@ def test_sixteen_rows_at_a_time_end_where_a_launch_does(L):
         return L.he_fp4_product_workspace_bytes(M, N, K, whole)
     assert wants(65535 * 16, 16, 100) == 0 and wants(65535 * 16 + 1, 16, 100) == (65535 * 16 + 1) * 128 * 2
     assert wants(65535 * 16, 16, 7) == 65535 * 16 * 128 * 2 and wants(1 << 22, 16, 128) == 0
+
+
+@pytest.mark.parametrize("whole", [0, 1])
+@pytest.mark.parametrize("N,K", [(3584, 18944), (3584, 3584), (37888, 3584), (1001, 1003), (512, 896), (130, 8200), (2048, 18944), (16, 65536), (300, 18950), (40, 5)])
+def test_a_workspace_serves_fewer_rows(L, N, K, whole):
+    """What is allocated for the largest batch is enough for every smaller one, and no more than the largest of their own."""
+    most = 0
+    for m in range(1, 1400):
+        most = max(most, L.he_fp4_product_call_bytes(m, N, K, whole))
+        assert L.he_fp4_product_workspace_bytes(m, N, K, whole) == most, m
+    # rows beyond those that are cut along K
+    for m in (5000, 20001, 200000):
+        assert L.he_fp4_product_workspace_bytes(m, N, K, whole) >= max(most, *(L.he_fp4_product_call_bytes(x, N, K, whole) for x in (m // 7, m // 3, m - 1, m)))
+
+
+def test_products_that_fewer_rows_cut_more_often(L):
+    """The sizes at which a workspace for one number of rows was not enough for one row less."""
+    for m in (32, 512):
+        assert L.he_fp4_product_call_bytes(m, 3584, 18944, 1) > L.he_fp4_product_call_bytes(m + 1, 3584, 18944, 1)
+        assert L.he_fp4_product_workspace_bytes(m + 1, 3584, 18944, 1) >= L.he_fp4_product_workspace_bytes(m, 3584, 18944, 1) > 0
+
+
+@pytest.mark.parametrize("top,experts,I,D", [(4, 16, 2048, 2048), (2, 8, 24, 72), (8, 200, 100, 36), (1, 2, 3, 5), (3, 64, 1000, 130)])
+def test_the_experts_workspace_serves_fewer_rows(L, top, experts, I, D):
+    sizes = [L.he_fp4_experts_workspace_bytes(m, top, experts, I, D) for m in range(3000)]
+    assert sizes == sorted(sizes)

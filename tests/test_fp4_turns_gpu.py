@@ -38,3 +38,20 @@ def test_more_rows_than_a_turn(M, N, K, apart):
         assert torch.equal(out[r0:r0 + n], first[:n])
     del room, out, ws
     torch.cuda.empty_cache()
+
+
+def test_one_workspace_for_every_number_of_rows():
+    """A server's: what 513 rows want serves all fewer ones, which are cut into more slices; the slices' memory is written before it is read."""
+    from hector_engine_amd.kernels import fp4, ops
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    N, K, M = 3584, 18944, 513
+    x, w = torch.randn((M, K), generator=gen, device="cuda").to(BF16), fp4.pack(torch.randn((N, K), generator=gen, device="cuda") * 0.05, 128)
+    values = w.unpack(F32).double()
+    want, size = x.double() @ values.T, (128 + 148 + 16) * 2.0 ** -23 * (x.double().abs() @ values.abs().T)      # (as fp4_plain.sum_bound)
+    ws = torch.full((ops.fp4_product_workspace_bytes(M, w, whole=True),), 0xFF, dtype=torch.uint8, device="cuda")
+    assert ops.fp4_product_workspace_bytes(M, w, whole=True, alone=True) < ops.fp4_product_workspace_bytes(M - 1, w, whole=True, alone=True)
+    for m in (513, 512, 65, 64, 33, 32, 17, 16, 1):
+        out = torch.full((m + 1, N), 7.0, device="cuda")
+        ws.fill_(0xFF)
+        ops.fp4_product(out, x, w, None, m, workspace=ws)
+        assert ((out[:m].double() - want[:m]).abs() <= size[:m] + 2.0 ** -24 * want[:m].abs()).all() and (out[m] == 7).all()
