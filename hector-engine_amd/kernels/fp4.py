@@ -65,6 +65,14 @@ class Fp4Weight:
     def dim(self) -> int:
         return len(self.shape)
 
+    def first_rows(self, rows: int) -> "Fp4Weight":
+        """The first rows of a matrix [N, K], whole tiles of 16 or all, over the same memory."""
+        n, *k = self._shape
+        if len(k) != 1 or not 0 < rows <= n or (rows % TILE_ROWS and rows != n):
+            raise ValueError(f"fp4: the first {rows} rows of {self._shape} are not whole tiles of {TILE_ROWS}")
+        tiles = -(-rows // TILE_ROWS)
+        return Fp4Weight(self._codes[:tiles], self._scales[:tiles], (rows, *k), self._group)
+
     def unpack(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, bfloat16 (exact) or float32."""
         from . import ops

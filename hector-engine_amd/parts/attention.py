@@ -67,7 +67,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ..kernels import kv_layout, ops, routes
+from ..kernels import fp4, kv_layout, ops, routes
 from .base import (BuildEnv, KVNeed, LayerCache, Mixer, PartSpec, PieceRows, StepContext, TensorSpec,
                    build_part, param, register_part, tensor_name)
 
@@ -342,6 +342,13 @@ class Attention(Mixer):
         # the fused one-token kernel's counters of finished workgroups (zeros between launches): its launches that cut the
         # keys across workgroups have few rows, as a rule fewer than a workgroup a compute unit
         self._arrived = torch.zeros(JOIN_COUNTERS, dtype=torch.int32, device=wo.device)
+
+    def pack_weights(self, group: int) -> None:
+        qkv, q = self.qkv, self.q_only
+        if qkv is not None and q.weight.data_ptr() == qkv.weight.data_ptr() and (q.out_features % fp4.TILE_ROWS == 0 or q.out_features == qkv.out_features):
+            qkv.pack(group)                # q's rows are the first of q||k||v, stored and packed
+            q.pack(group, qkv.weight.first_rows(q.out_features))
+        super().pack_weights(group)
 
     def _by_map(self, which: str, t: torch.Tensor) -> torch.Tensor:
         """A differential attention's stored rows (or bias) as the kernels' heads read them: q from

@@ -83,10 +83,11 @@ class Linear:
         """Whether the weight is in 4 bits."""
         return isinstance(self.weight, fp4.Fp4Weight)
 
-    def pack(self, group: int) -> None:
-        """The weight in 4 bits from here on (kernels.fp4), where the part allows it; the stored one is let go."""
+    def pack(self, group: int, packed: fp4.Fp4Weight | None = None) -> None:
+        """The weight in 4 bits from here on (kernels.fp4), where the part allows it; the stored one is let go. packed: it is there already, as rows
+        of another layer's."""
         if self.packable and not self.packed:
-            self.weight = fp4.pack(self.weight, group)
+            self.weight = fp4.pack(self.weight, group) if packed is None else packed
             self._plans.clear()
             self._chosen.clear()
 

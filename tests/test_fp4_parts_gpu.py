@@ -109,3 +109,48 @@ def test_the_last_rows_of_a_long_step(tail, ordered):
     for lin in (part.gate_up, part.down):
         lin.pack(64)
     assert torch.equal(part.forward(x, context(rows))[8192:rows], part.forward(last, context(tail))[:tail])
+
+
+def test_the_first_rows_of_a_packed_matrix():
+    from hector_engine_amd.kernels import fp4, ops
+    w = torch.randn((100, 264), generator=torch.Generator().manual_seed(4)).cuda()
+    packed = fp4.pack(w, 32)
+    for rows in (16, 48, 96, 100):
+        first = packed.first_rows(rows)
+        assert first.pointers == packed.pointers and torch.equal(first.unpack(), packed.unpack()[:rows])
+        x = torch.randn((5, 264), generator=torch.Generator().manual_seed(5)).to(BF16).cuda()
+        whole, own = torch.empty((5, 100), device="cuda"), torch.full((6, rows), 7.0, device="cuda")
+        ops.fp4_product(whole, x, packed, None, 5)
+        ops.fp4_product(own, x, first, None, 5)
+        assert torch.equal(own[:5], whole[:, :rows]) and (own[5] == 7).all()
+    for rows in (0, -16, 8, 99, 112):
+        with pytest.raises(ValueError, match="whole tiles of 16"):
+            packed.first_rows(rows)
+    with pytest.raises(ValueError, match="whole tiles of 16"):
+        fp4.pack(w[None], 32).first_rows(16)
+
+
+def linears(model):
+    from hector_engine_amd.parts.linear import Linear
+    todo = list(model.parts())
+    while todo:
+        p = todo.pop()
+        yield from ((p, name, lin) for name, lin in vars(p).items() if isinstance(lin, Linear))
+        todo += p.children()
+
+
+@pytest.mark.parametrize("name", ["A", "B", "C", "D"])
+def test_packed_matrices_are_held_once(model_dirs, name):
+    """What a packed engine holds of its layers' matrices is q||k||v, o, gate||up and down: q's rows alone are the first of q||k||v, as they are with stored weights."""
+    import hector_engine_amd as he
+    from hector_engine_amd.kernels import fp4
+    eng = he.Engine(model_dirs[name], weights="fp4", weight_group=32, dtype="bfloat16", max_tokens=256, max_slots=2, max_seq_len=64)
+    held, sizes = {}, 0
+    for part, attr, lin in linears(eng.model):
+        if lin.packed:
+            for t in (lin.weight.codes, lin.weight.scales):
+                held[t.untyped_storage().data_ptr()] = t.untyped_storage().nbytes()
+            if attr != "q_only":
+                codes, scales = fp4.storage_shapes((lin.out_features, lin.in_features), 32)
+                sizes += torch.Size(codes).numel() + 2 * torch.Size(scales).numel()
+    assert sum(held.values()) == sizes > 0
