@@ -1571,6 +1571,16 @@ def fp4_product_carried(out, x, w, bias, rows: int, *, gated: bool = False, act=
         F32 if bias is None else dtype_code(bias.dtype), gated, *_act4(act), owed, count, float(eps), *resid, _stream()))
 
 
+FP4_MOST_EXPERTS = 1024
+
+
+def fp4_experts_most_rows(top: int, down) -> int:
+    """The rows that a call of fp4_experts takes: the choices' activations and the rows span less than 4 GiB, in whole blocks of 128 values."""
+    E, D, I = down.shape
+    blocks = lambda n: -(-n // 128) * 128
+    return min(65535, ((1 << 26) - 1) // top, ((1 << 31) - 1) // (top * blocks(I)), ((1 << 31) - 1) // blocks(D))
+
+
 def fp4_experts_workspace_bytes(rows: int, top: int, gate_up, down) -> int:
     """Bytes of scratch memory that fp4_experts wants for so many rows of `top` choices."""
     E, D, I = down.shape
@@ -1582,7 +1592,7 @@ def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0
     """A routed feed-forward over packed experts: out[rows, D] (bfloat16) = the sum over a row's choices c of weights[row, c] *
     down[e] act(gate[e] x, up[e] x) with e = ids[row, c]; an id that is no expert adds nothing, nor does a weight of 0; with identity an id from E on adds
     weights[row, c] * x. gate_up: packed [E, 2 I, D], gate i of an expert in row 2 i, its up in 2 i + 1; down: packed [E, D, I]; ids int32, weights float32
-    [rows, top]; x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. plus: float32 [rows, D], added to the sums before they are
+    [rows, top], E up to 1024, rows up to fp4_experts_most_rows(top, down); x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. plus: float32 [rows, D], added to the sums before they are
     rounded (what a shared expert gives). workspace: uint8,
     fp4_experts_workspace_bytes(rows, top, gate_up, down) or more; calls that may run at the same time need one each."""
     device = _fp4_weight("fp4_experts", gate_up, 3)

@@ -158,6 +158,8 @@ class RoutedExperts(FeedForward):
 
     def pack_weights(self, group: int) -> None:
         E, I, S, D = self.real, self.inter, self.shared_cols, self.hidden
+        if E > ops.FP4_MOST_EXPERTS:
+            raise ValueError(f"{self.prefix}: {E} experts cannot be packed into 4 bits, {ops.FP4_MOST_EXPERTS} at most")
         up, down = self.gate_up.weight, self.down.weight
         experts = (fp4.pack(up[:2 * E * I].view(E, 2 * I, D), group),
                    fp4.pack(down[:, :E * I].view(D, E, I).transpose(0, 1).contiguous(), group))
@@ -173,8 +175,9 @@ class RoutedExperts(FeedForward):
         up, down, shared = self.packed
         rows, act = ctx.rows, (self.alpha, self.limit, self.up_shift)
         out = ctx.alloc((rows, self.hidden))
-        for r0 in range(0, rows, _ROW_CHUNK):
-            n = min(_ROW_CHUNK, rows - r0)
+        most = min(_ROW_CHUNK, ops.fp4_experts_most_rows(self.top, down))
+        for r0 in range(0, rows, most):
+            n = min(most, rows - r0)
             turn = ctx.scratch.mark()
             common = None
             if shared is not None:

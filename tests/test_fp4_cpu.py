@@ -171,3 +171,31 @@ def test_products_that_fewer_rows_cut_more_often(L):
 def test_the_experts_workspace_serves_fewer_rows(L, top, experts, I, D):
     sizes = [L.he_fp4_experts_workspace_bytes(m, top, experts, I, D) for m in range(3000)]
     assert sizes == sorted(sizes)
+
+
+class OfShape:
+    def __init__(self, *shape):
+        self.shape = shape
+
+
+@pytest.mark.parametrize("top,D,I", [(4, 2048, 2048), (8, 256, 65536), (64, 100, 20000), (1, 1 << 20, 300), (2000, 64, 16)])
+def test_the_most_rows_of_the_experts(L, top, D, I):
+    """What the engine takes for a call's most rows is what the operator takes."""
+    from hector_engine_amd.kernels import ops
+    most = ops.fp4_experts_most_rows(top, OfShape(2, D, I))
+
+    def call(rows):
+        return refusal(L, L.he_fp4_experts(AT, AT, D, AT, AT, AT, AT, AT, AT, rows, top, 2, I, D, 32, 32, 0, 1.0, 0.0, 0.0, 0.0, None, 0, None))
+    assert "a workspace of" in call(most) and "too many" in call(most + 1)
+
+
+def test_more_experts_than_the_operator_takes_are_not_packed():
+    """Refused when the model's weights are packed, not by its first step."""
+    from hector_engine_amd.kernels import ops
+    from hector_engine_amd.parts.base import BuildEnv, PartSpec, build_part
+    from hector_engine_amd.parts.linear import Linear
+    part = build_part("feed_forward", PartSpec("routed_experts", {"hidden_size": 8, "intermediate_size": 8, "experts": ops.FP4_MOST_EXPERTS + 1, "top": 2}), "m.",
+                      BuildEnv(torch.device("cpu"), torch.bfloat16, True))
+    part.gate_up, part.down = (Linear(torch.empty(s, dtype=torch.bfloat16, device="meta")) for s in ((16 * part.real, 8), (8, 8 * part.real)))
+    with pytest.raises(ValueError, match="1025 experts cannot be packed"):
+        part.pack_weights(32)
