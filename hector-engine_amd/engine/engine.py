@@ -123,8 +123,8 @@ class Engine:
         multiple of 256 and at most this and they want at most 64 places (fixed prompt chunks; 0,
         or graph_step_rows 0: none).
         weights: "stored", or "fp4": the layers' matrices are packed into 4 bits when they are loaded, in groups of `weight_group`
-        (32, 64 or 128) along K that share a scale (kernels/fp4.py), and read so by every step; bfloat16 engines only. The
-        embedding, the norms, routers and gates and the output head stay as they are stored. (The reference serves its
+        (32, 64 or 128) along K that share a scale (kernels/fp4.py), and read so by every step; bfloat16 engines only. What is
+        packed, and what stays as it is stored: DecoderModel.pack_weights. (The reference serves its
         models in formats of 4 to 5 bits: tools/quant_bench/README.md:305-307.)
         sync_each_launch: a debugging mode (the reference's sync_after_each_op, src/engine.cpp:318-334):
         steps run without HIP graphs and the host waits for the GPU after every launch, so that

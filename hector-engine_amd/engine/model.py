@@ -87,7 +87,11 @@ class DecoderModel:
         self._keep_orders()
 
     def pack_weights(self, group: int) -> None:
-        """The layers' product weights in 4 bits (kernels.fp4); embedding, norms, routers, gates and the head stay as they are."""
+        """The layers' product weights in 4 bits (kernels.fp4): attention's q||k||v and o, feed-forwards' and experts' matrices, the memories' and the delta
+        rule's q||k||v||g and o, a state space's in and out matrices, latent attention's projections into and out of its ranks, a token input's two; and with
+        them the rows that ride in these: output gates (of attention, latent attention, the memories, the delta rule) and a state space's dt. As they are
+        stored stay the embedding and other tables, norms, routers, biases, convolutions, a shared expert's gate vector, the gates that a
+        matrix memory and a delta rule forget and write by, latent attention's matrices of a head (w_keys, w_values: batched products), and the output head."""
         todo = list(self.parts())
         while todo:
             p = todo.pop()

@@ -3,6 +3,8 @@ import pytest
 import torch
 
 from tests.plain import fp4_plain as P
+from tests.test_fp4_engine_gpu import (bobevik_folders, butolorn_folders, dofipel_folders, domorax_folders, penasun_folders,  # noqa: F401
+                                       volonex_folders)
 from tests.test_fp4_gpu import experts_case, workspace
 from tests.test_tile_routes_gpu import bound_part, context
 
@@ -154,3 +156,36 @@ def test_packed_matrices_are_held_once(model_dirs, name):
                 codes, scales = fp4.storage_shapes((lin.out_features, lin.in_features), 32)
                 sizes += torch.Size(codes).numel() + 2 * torch.Size(scales).numel()
     assert sum(held.values()) == sizes > 0
+
+
+# What each design's layers hold as matrices of products: packed, as they are stored.
+ATTENTION, LATENT = {"Attention.qkv", "Attention.q_only", "Attention.o_proj"}, {"LatentAttention.front", "LatentAttention.o_proj"}
+GATED, DENSE = {"GatedMLP.gate_up", "GatedMLP.down"}, {"DenseMLP.up", "DenseMLP.down"}
+PACKED = {"bobevik": (ATTENTION | GATED | {"DecayMemory.qkvg", "DecayMemory.o_proj"}, set()),
+          "butolorn": (ATTENTION | DENSE | {"GatedTokenInput.gate", "GatedTokenInput.proj", "MatrixMemory.qkvg", "MatrixMemory.o_proj"}, {"MatrixMemory.gates"}),
+          "dofipel": (ATTENTION | LATENT | GATED | {"LatentAttention.front_q"}, {"LatentAttention.w_keys", "LatentAttention.w_values", "RoutedExperts.router"}),
+          "domorax": (ATTENTION | LATENT | GATED | DENSE | {"LatentAttention.dq", "LatentAttention.uq", "GatedDeltaRule.qkvg", "GatedDeltaRule.o_proj"},
+                      {"GatedDeltaRule.gates", "LatentAttention.w_keys", "LatentAttention.w_values", "RoutedExperts.router"}),
+          "penasun": (ATTENTION | {"SelectiveScanMixer.in_proj", "SelectiveScanMixer.o_proj"}, {"RoutedExperts.router"}),
+          "volonex": (ATTENTION | GATED, set())}
+
+
+@pytest.mark.parametrize("design", sorted(PACKED))
+def test_what_is_packed(request, design):
+    import hector_engine_amd as he
+    from hector_engine_amd.parts.routed import RoutedExperts
+    from tests.test_fp4_engine_gpu import DESIGNS, OPTS, parts_of
+    folders = request.getfixturevalue(f"{design}_folders")
+    packed, stored = set(), set()
+    for name in sorted(DESIGNS[design]):
+        eng = he.Engine(folders[name + "_calm" if name + "_calm" in folders else name], weights="fp4", weight_group=32, **OPTS)
+        for part, attr, lin in linears(eng.model):
+            (packed if lin.packed else stored).add(f"{type(part).__name__}.{attr}")
+            assert lin.packed or isinstance(lin.weight, torch.Tensor)
+        for part in parts_of(eng.model):
+            if isinstance(part, RoutedExperts):
+                assert part.packed is not None and part.gate_up is None and part.down is None
+            for attr in ("router", "w_keys", "w_values"):
+                if isinstance(getattr(part, attr, None), torch.Tensor):
+                    stored.add(f"{type(part).__name__}.{attr}")
+    assert (packed, stored) == (PACKED[design][0], PACKED[design][1] | {"LinearHead.linear"})
