@@ -299,6 +299,9 @@ extern "C" int he_fp4_experts_plus(void* out, const void* x, int64_t ldx, const 
   GroupRows lists = {};
   int rc = 0;
   if (!by_ids && (rc = he_group_rows(&lists, p, ids_i32, weights_f32, rows, top, experts, t.bm, stream))) return rc;
+  // The activations times their share are rounded to bfloat16, the second product's operands: half a step, 2^-8 of each at most. The results are 0.0023 to 0.0024 of their
+  // size from 64 bits, 0.0017 with 32 bits between the products (1, 64 and 2048 rows of 16 experts of 2048). Two operands a value would take the rounding away and
+  // double the second product's matrix instructions (2048 rows: 94 of 264 us).
   uint16_t* h = (uint16_t*)(p + t.ints);
   float* partial = (float*)(p + t.ints + t.h);
   up.x = (const uint16_t*)x, up.ldx = ldx, up.whole = whole_rows(x, ldx), up.M = rows;

@@ -23,8 +23,9 @@ __device__ __forceinline__ void fixed() { __builtin_amdgcn_sched_barrier(0); }
 // the row, so that the rows of an operand are in different banks. The codes come into registers one block ahead, each a value of bfloat16 before
 // it is multiplied. (Scales by way of LDS too: 32 rows of 18944 x 3584 15 -> 19 us.)
 // 2048 x 37888 x 3584 gated 457 us (1.22 PFLOP/s): matrix cores 0.57 of the cycles, the other vector instructions, 256 of 296 a block for the
-// conversions, 0.38, and the two do not overlap. Tiles of 64 rows and fewer are bound by what a unit takes in, some 50 GB/s: the rows again for
-// every tile of columns.
+// conversions, 0.38, and the two do not overlap. Tiles of 64 rows and fewer wait: a block takes some 1 us (64 rows of 37888 x 3584 28 of them in 27 to
+// 30 us, 203 of 4608 x 3584 14 a part in 15 to 17), matrix cores 0.20 and other vector instructions 0.26 of the cycles: each block is asked for one ahead and waited for
+// whole, so a unit has some 47 KB on their way at a time. (Tiles of more columns, which read the rows less often, were no faster.)
 template <int MT, int NT, int PARTS, int GROUPS>
 __global__ __launch_bounds__(256 * PARTS, PARTS == 1 ? 2 : 1) void fp4_tall_kernel(Fp4Case c, int mtiles, int ntiles, int slices, float* __restrict__ sums) {
   constexpr int BM = 16 * MT, BLOCK = BM * 256;            // bytes of a block of X

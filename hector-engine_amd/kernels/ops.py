@@ -1593,7 +1593,7 @@ def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0
     down[e] act(gate[e] x, up[e] x) with e = ids[row, c]; an id that is no expert adds nothing, nor does a weight of 0; with identity an id from E on adds
     weights[row, c] * x. gate_up: packed [E, 2 I, D], gate i of an expert in row 2 i, its up in 2 i + 1; down: packed [E, D, I]; ids int32, weights float32
     [rows, top], E up to 1024, rows up to fp4_experts_most_rows(top, down); x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. plus: float32 [rows, D], added to the sums before they are
-    rounded (what a shared expert gives). workspace: uint8,
+    rounded (what a shared expert gives). The activations times their weights are rounded to bfloat16 between the two products. workspace: uint8,
     fp4_experts_workspace_bytes(rows, top, gate_up, down) or more; calls that may run at the same time need one each."""
     device = _fp4_weight("fp4_experts", gate_up, 3)
     _fp4_weight("fp4_experts", down, 3)
