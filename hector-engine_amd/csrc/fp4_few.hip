@@ -8,6 +8,22 @@ struct __attribute__((packed, aligned(2))) Piece {
   uint4 v;
 };
 
+// sum + a block of 128 k with the scales in the operands: a lane's codes, scales, row of X, and its first k
+template <int GROUPS>
+__device__ __noinline__ fp4_f32x4 scaled_block(fp4_f32x4 sum, const uint8_t* codes, const uint16_t* scales, const uint16_t* row, int k, int K) {
+#pragma unroll 1
+  for (int t = 0; t < 4; ++t, k += 32) {
+    uint32_t words[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < K) words[e >> 1] |= (uint32_t)row[k + e] << (16 * (e & 1));
+    const fp4_bf16x8 v = __builtin_bit_cast(fp4_bf16x8, make_uint4(words[0], words[1], words[2], words[3]));
+    const uint32_t scale = scales[t * GROUPS / 4 * 16];
+    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_values(*reinterpret_cast<const uint32_t*>(codes + 4 * t), __uint_as_float(scale << 16)), v, sum, 0, 0, 0);
+  }
+  return sum;
+}
+
 enum { ROWS_ALONE, CHOICES, NORM };
 
 // A workgroup has NT tiles of 16 weight rows; its W wavefronts cut K among them, and their sums meet in LDS. Codes, scales and X (4 XL rows of it)
@@ -208,9 +224,9 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
 #pragma unroll
   for (int j = 0; j < NT; ++j) *reinterpret_cast<fp4_f32x4*>(own + j * 1024 + lane * 16) = acc[j];
   // A group's sum of x * code can leave the range of 32 bits where its scaled one does not (128 values of x from 4.4e35 on): a wavefront that ends with infinities
-  // or NaN takes those sums once more with the scales in the operands, as the kernel of many rows has them. (One tile after the other, each value by itself: with the
+  // or NaN takes those sums once more with the scales in the operands, as the kernel of many rows has them. (One block after the other in a function of its own: with the
   // loads of the loop above the kernels held so many more registers that 16 rows of 37888 x 3584 in groups of 32 took 26.3 us, 22.4 without; so 63 products of 1 to
-  // 16 rows take 1.008 of the time without in the geometric mean.)
+  // 16 rows take 1.003 of the time without in the geometric mean.)
   bool off = false;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -222,21 +238,12 @@ __global__ __launch_bounds__(64 * W) void fp4_few_kernel(Fp4Case c) {
     for (int j = 0; j < NT; ++j) {
       fp4_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-      for (int step = 4 * lo; step < 4 * hi; ++step) {     // of 32 k
-        const int unit = step >> 2, t = step & 3, choice = CHAIN ? unit / blocks : 0, kb = unit - choice * blocks;
+      for (int unit = lo; unit < hi; ++unit) {
+        const int choice = CHAIN ? unit / blocks : 0, kb = unit - choice * blocks;
         const int expert = CHAIN ? __builtin_amdgcn_readlane(id, choice) : group;
         if (expert < 0) continue;
         const int64_t at = ((int64_t)expert * c.w.tiles + min(tile0 + j, c.w.tiles - 1)) * blocks + kb;
-        const uint32_t codes = *reinterpret_cast<const uint32_t*>(c.w.codes + at * FP4_TILE_BYTES + lane * 16 + 4 * t);
-        const uint32_t scale = c.w.scales[at * (16 * GROUPS) + t * GROUPS / 4 * 16 + r16];
-        const int k = kb * FP4_K + 32 * t + 8 * kq;
-        const uint16_t* p = row + choice * c.ldx + k;
-        uint32_t words[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + e < K) words[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
-        const fp4_bf16x8 v = __builtin_bit_cast(fp4_bf16x8, make_uint4(words[0], words[1], words[2], words[3]));
-        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_values(codes, __uint_as_float(scale << 16)), v, sum, 0, 0, 0);
+        sum = scaled_block<GROUPS>(sum, c.w.codes + at * FP4_TILE_BYTES + lane * 16, c.w.scales + at * (16 * GROUPS) + r16, row + choice * c.ldx, kb * FP4_K + 8 * kq, K);
       }
       fp4_f32x4 kept = *reinterpret_cast<const fp4_f32x4*>(own + j * 1024 + lane * 16);
 #pragma unroll
