@@ -1488,7 +1488,8 @@ def fp4_product_workspace_bytes(rows: int, w, gated: bool = False, whole: bool =
 def fp4_product(out, x, w, bias, rows: int, *, gated: bool = False, act=_SILU, workspace=None) -> None:
     """out[rows, N] (bfloat16 or float32) = x[rows, K] (bfloat16) . W^T (+ bias [N]) with a packed weight (kernels.fp4), sums in 32 bits;
     or, gated, out[rows, N / 2] (bfloat16, no bias) = act(gate, up) for a weight that alternates gate and up rows, act =
-    (alpha, limit, up_shift[, cubic]) the activation's constants as silu_mul takes them. The rows of x and out may lie apart.
+    (alpha, limit, up_shift[, cubic]) the activation's constants as silu_mul takes them. The rows of x and out may lie apart; out shares no memory
+    with x. Up to 2^22 rows.
     workspace: uint8, fp4_product_workspace_bytes(rows, w) or more, which serves calls of fewer rows too; calls that may run at the same time need one each."""
     device = _fp4_weight("fp4_product", w, 2)
     N, K = w._shape
@@ -1528,7 +1529,7 @@ def fp4_product_carried(out, x, w, bias, rows: int, *, gated: bool = False, act=
     """fp4_product of up to 16 rows (K 8 at least) that an RMS norm is carried across. row_scale = (partials float32 [rows or more, count], eps): the rows of
     x are r * gain of a norm whose 1 / sqrt(mean(r^2) + eps) is applied to the sums here (mean over K). residual = (resid float32 [rows or more, N],
     gain [N], xg bfloat16, squares float32 [rows or more, ceil(N / 16)][, scale]): instead of writing `out` (None), resid += scale * result in place,
-    xg = resid * gain, squares = the sums of resid^2 over sixteen columns (N a multiple of 4)."""
+    xg = resid * gain, squares = the sums of resid^2 over sixteen columns (N a multiple of 4). What is written shares no memory with x."""
     device = _fp4_weight("fp4_product_carried", w, 2)
     N, K = w.shape
     if not 0 <= rows <= FP4_CARRIED_ROWS or K < 8:
@@ -1593,7 +1594,7 @@ def fp4_experts(out, x, gate_up, down, ids, weights, rows: int, *, act=(1.0, 0.0
     down[e] act(gate[e] x, up[e] x) with e = ids[row, c]; an id that is no expert adds nothing, nor does a weight of 0; with identity an id from E on adds
     weights[row, c] * x. gate_up: packed [E, 2 I, D], gate i of an expert in row 2 i, its up in 2 i + 1; down: packed [E, D, I]; ids int32, weights float32
     [rows, top], E up to 1024, rows up to fp4_experts_most_rows(top, down); x bfloat16 [rows, D], its rows may lie apart; act as fp4_product takes it. plus: float32 [rows, D], added to the sums before they are
-    rounded (what a shared expert gives). The activations times their weights are rounded to bfloat16 between the two products. workspace: uint8,
+    rounded (what a shared expert gives). out shares no memory with x or plus. The activations times their weights are rounded to bfloat16 between the two products. workspace: uint8,
     fp4_experts_workspace_bytes(rows, top, gate_up, down) or more; calls that may run at the same time need one each."""
     device = _fp4_weight("fp4_experts", gate_up, 3)
     _fp4_weight("fp4_experts", down, 3)
