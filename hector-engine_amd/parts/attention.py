@@ -345,7 +345,8 @@ class Attention(Mixer):
 
     def pack_weights(self, group: int) -> None:
         qkv, q = self.qkv, self.q_only
-        if qkv is not None and q.weight.data_ptr() == qkv.weight.data_ptr() and (q.out_features % fp4.TILE_ROWS == 0 or q.out_features == qkv.out_features):
+        if qkv is not None and qkv.packable and not qkv.packed and q.weight.data_ptr() == qkv.weight.data_ptr() \
+                and (q.out_features % fp4.TILE_ROWS == 0 or q.out_features == qkv.out_features):
             qkv.pack(group)                # q's rows are the first of q||k||v, stored and packed
             q.pack(group, qkv.weight.first_rows(q.out_features))
         super().pack_weights(group)

@@ -156,6 +156,9 @@ def test_packed_matrices_are_held_once(model_dirs, name):
                 codes, scales = fp4.storage_shapes((lin.out_features, lin.in_features), 32)
                 sizes += torch.Size(codes).numel() + 2 * torch.Size(scales).numel()
     assert sum(held.values()) == sizes > 0
+    before = [lin.weight for _, _, lin in linears(eng.model)]
+    eng.model.pack_weights(32)                       # (packed already: nothing changes)
+    assert all(a is lin.weight for a, (_, _, lin) in zip(before, linears(eng.model)))
 
 
 # What each design's layers hold as matrices of products: packed, as they are stored.
